@@ -5,6 +5,7 @@ RuntimeError: there is no CPU fallback for any op in this package.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import threading
 from pathlib import Path
@@ -29,6 +30,19 @@ SIGNATURES: dict[str, list] = {
     "fk_rmsnorm_bwd_workspace_size": [_i64, _i64, C.POINTER(_sz)],
     "fk_rmsnorm_bwd": [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i32, _vp],
     "fk_rmsnorm_bwd_noalloc": [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i32, _vp],
+    "fk_add_rmsnorm_fwd": [_vp, _i64, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _f32,
+                           _i32, _vp],
+    "fk_add_rmsnorm_bwd_workspace_size": [_i64, _i64, C.POINTER(_sz)],
+    "fk_add_rmsnorm_bwd": [_vp, _i64, _vp, _i64, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp,
+                           _sz, _i64, _i64, _i32, _vp],
+    "fk_add_rmsnorm_quant": [_vp, _i64, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _i64,
+                             _i64, _f32, _i32, _vp],
+    "fk_moe_balance_workspace_size": [C.POINTER(_sz)],
+    "fk_moe_balance": [_vp, _i64, _vp, _vp, _i64, _i32, _i32, _f32, _f32, _vp, _vp, _vp, _vp, _sz,
+                       _i32, _vp],
+    "fk_distill_workspace_size": [_i64, _i32, C.POINTER(_sz)],
+    "fk_distill": [_vp, _i64, _vp, _i64, _vp, _vp, _i32, _i32, _vp, _i64, _i64, _i64, _f32, _f32,
+                   _f32, _i32, _vp, _vp, _vp, _sz, _vp],
     "fk_router_fwd": [_vp, _i64, _i32, _i64, _i32, _i32, _vp, _vp, _vp],
     "fk_router_bwd": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp],
     "fk_ce_fwd": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _f32, _i32, _vp, _vp, _vp, _vp,
@@ -173,6 +187,65 @@ def moe_capacity(n_tokens: int, k: int, n_experts: int) -> tuple[int, int]:
               "fk_moe_capacity")
         v = _cap_cache[key] = (rows.value, ws.value)
     return v
+
+
+_op_ws_cache: dict = {}
+
+
+def workspace_bytes(name: str, device: torch.device, *sizes) -> int:
+    """Bytes that the sizing entry point ``name`` gives for these sizes on ``device``."""
+    key = (name, device.index, *sizes)
+    v = _op_ws_cache.get(key)
+    if v is None:
+        if len(_op_ws_cache) >= 4096:  # batches of ever new lengths: start over
+            _op_ws_cache.clear()
+        out = C.c_size_t(0)
+        with torch.cuda.device(device):
+            check(getattr(load(), name)(*sizes, C.byref(out)), name)
+        v = _op_ws_cache[key] = out.value
+    return v
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor):
+    """Context in which launches go to ``t``'s device (free where it is the current one)."""
+    i = t.device.index
+    return _NO_SWITCH if i == torch.cuda.current_device() else torch.cuda.device(i)
+
+
+def rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """``t`` as [rows, cols] with unit stride along a row and rows that do not overlap
+    (a view where there is one)."""
+    t = t.reshape(-1, cols)
+    if t.shape[0] > 1 and t.stride(0) < cols or cols > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t
+
+
+def row_stride(t: torch.Tensor) -> int:
+    """Row stride of a [rows, cols] tensor from rows_of, in elements (a tensor of one row
+    may report any stride)."""
+    return max(t.stride(0), t.shape[1])
+
+
+def hand_over_gradient(ctx, grad_output: torch.Tensor) -> torch.Tensor:
+    """The gradient that a forward pass already computed (ctx.grad, for grad_output ==
+    ctx.loss_scale), scaled in place where grad_output is another number: the device decides,
+    without a host sync.  It is the caller's from here on, so it is given once."""
+    grad = ctx.grad
+    if grad is None:
+        raise RuntimeError("the gradient of this loss was handed over in its first backward "
+                           "pass: compute the loss again for another one")
+    ctx.grad = None
+    go = grad_output.to(torch.float32)
+    if ctx.loss_scale != 1.0:
+        go = go / ctx.loss_scale
+    with on_device(grad):
+        call("fk_ce_bwd_scale", grad.data_ptr(), row_stride(grad), grad.shape[0], grad.shape[1],
+             go.data_ptr(), dtype_code(grad.dtype), stream_of(grad))
+    return grad.detach()
 
 
 def num_sms(device: torch.device | None = None) -> int:

@@ -1,0 +1,299 @@
+// Residual addition + RMSNorm: forward, backward, and a forward with an 8-bit output.
+//
+//   h = round_R(x + r),  s = rsqrt(mean(h^2) + eps),  y = round_T(h * s * w)
+//   given dy, dh:  g = dh + s*w*dy - h * s^3 * mean(w*dy*h),  dx = round_T(g),
+//   dr = round_R(g),  dw = sum_rows dy*h*s
+//   8 bits: per group of columns  scale = max(max|h*s*w| / 448, 2^-126),
+//   q = e4m3(h*s*w / scale) with the fp32 product h*s*w, not its rounding to T.
+//
+// The norm is taken of the rounded sum h, the tensor that is stored and that the backward
+// reads, so forward and backward see the same row.  T is the type of x and y, R the type
+// of the residual stream (T or fp32); every statistic is fp32.
+#include "common.cuh"
+
+#include <cuda_fp8.h>
+
+namespace fk {
+namespace {
+
+constexpr float kE4m3Max = 448.f;
+constexpr float kMinScale = 1.17549435e-38f;  // 2^-126: a row of zeros keeps a usable scale
+
+__device__ __forceinline__ float load_wd(const void* w, int wd, int64_t c) {
+  if (wd == FK_F32) return static_cast<const float*>(w)[c];
+  if (wd == FK_F16) return Elt<__half>::to_f(static_cast<const __half*>(w)[c]);
+  return Elt<__nv_bfloat16>::to_f(static_cast<const __nv_bfloat16*>(w)[c]);
+}
+
+__device__ __forceinline__ float block_sum(float v, float* red /*[32]*/) {
+  v = warp_sum(v);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+  __syncthreads();
+  if (lane == 0) red[warp] = v;
+  __syncthreads();
+  float s = 0.f;
+  for (int i = 0; i < nwarps; ++i) s += red[i];  // fixed order: deterministic
+  return s;
+}
+__device__ __forceinline__ float block_max(float v, float* red) {
+  v = warp_max(v);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+  __syncthreads();
+  if (lane == 0) red[warp] = v;
+  __syncthreads();
+  float m = red[0];
+  for (int i = 1; i < nwarps; ++i) m = fmaxf(m, red[i]);
+  return m;
+}
+
+// ------------------------------------------------------------------ any shape -----------
+// One CTA per row, element loops.  h is re-read by the thread that wrote it.
+template <typename T, typename R>
+__global__ void __launch_bounds__(256) add_rmsnorm_fwd_generic(
+    const T* __restrict__ x, int64_t xs, const R* __restrict__ r, int64_t rs,
+    const void* __restrict__ w, int wd, T* __restrict__ y, R* h, float* __restrict__ rstd,
+    int64_t rows, int64_t cols, float eps) {
+  __shared__ float red[32];
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    float ss = 0.f;
+    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) {
+      const R hv = Elt<R>::from_f(Elt<T>::to_f(x[row * xs + c]) + Elt<R>::to_f(r[row * rs + c]));
+      h[row * cols + c] = hv;
+      const float f = Elt<R>::to_f(hv);
+      ss = fmaf(f, f, ss);
+    }
+    const float s = rsqrtf(block_sum(ss, red) / (float)cols + eps);
+    if (threadIdx.x == 0 && rstd) rstd[row] = s;
+    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x)
+      y[row * cols + c] = Elt<T>::from_f(Elt<R>::to_f(h[row * cols + c]) * s * load_wd(w, wd, c));
+  }
+}
+
+template <typename T, typename R>
+__global__ void __launch_bounds__(256) add_rmsnorm_bwd_generic(
+    const T* __restrict__ dy, int64_t dys, const R* __restrict__ dh, int64_t dhs,
+    const R* __restrict__ h, const void* __restrict__ w, int wd, const float* __restrict__ rstd,
+    T* __restrict__ dx, R* __restrict__ dr, float* __restrict__ part, int64_t rows,
+    int64_t cols) {
+  __shared__ float red[32];
+  float* prow = part + (int64_t)blockIdx.x * cols;
+  for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) prow[c] = 0.f;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const float s = rstd[row];
+    float dot = 0.f;
+    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) {
+      const float d = Elt<T>::to_f(dy[row * dys + c]), hv = Elt<R>::to_f(h[row * cols + c]);
+      dot = fmaf(load_wd(w, wd, c) * d, hv, dot);
+      prow[c] = fmaf(d * hv, s, prow[c]);  // each column is one thread's
+    }
+    const float c2 = s * s * s * (block_sum(dot, red) / (float)cols);
+    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) {
+      const float d = Elt<T>::to_f(dy[row * dys + c]), hv = Elt<R>::to_f(h[row * cols + c]);
+      float g = s * (load_wd(w, wd, c) * d) - hv * c2;
+      if (dh) g += Elt<R>::to_f(dh[row * dhs + c]);
+      dx[row * cols + c] = Elt<T>::from_f(g);
+      if (dr) dr[row * cols + c] = Elt<R>::from_f(g);
+    }
+  }
+}
+
+__device__ __forceinline__ uint8_t to_e4m3(float v) {
+  return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+}
+
+// r == nullptr: h is x itself and is not written.
+template <typename T, typename R>
+__global__ void __launch_bounds__(256) add_rmsnorm_quant_generic(
+    const T* __restrict__ x, int64_t xs, const R* __restrict__ r, int64_t rs,
+    const void* __restrict__ w, int wd, uint8_t* __restrict__ q, float* __restrict__ scales,
+    R* h, int64_t rows, int64_t cols, int64_t block, float eps) {
+  __shared__ float red[32];
+  const int64_t groups = (cols + block - 1) / block;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    float ss = 0.f;
+    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) {
+      float f = Elt<T>::to_f(x[row * xs + c]);
+      if (r) {
+        const R hv = Elt<R>::from_f(f + Elt<R>::to_f(r[row * rs + c]));
+        h[row * cols + c] = hv;
+        f = Elt<R>::to_f(hv);
+      }
+      ss = fmaf(f, f, ss);
+    }
+    const float s = rsqrtf(block_sum(ss, red) / (float)cols + eps);
+    __syncthreads();  // the groups below read columns that other threads wrote
+    auto value = [&](int64_t c) {
+      const float f = r ? Elt<R>::to_f(h[row * cols + c]) : Elt<T>::to_f(x[row * xs + c]);
+      return f * s * load_wd(w, wd, c);
+    };
+    for (int64_t g = 0; g < groups; ++g) {
+      const int64_t c0 = g * block, c1 = c0 + block < cols ? c0 + block : cols;
+      float m = 0.f;
+      for (int64_t c = c0 + threadIdx.x; c < c1; c += blockDim.x) m = fmaxf(m, fabsf(value(c)));
+      const float scale = fmaxf(block_max(m, red) / kE4m3Max, kMinScale);
+      if (threadIdx.x == 0) scales[row * groups + g] = scale;
+      for (int64_t c = c0 + threadIdx.x; c < c1; c += blockDim.x)
+        q[row * cols + c] = to_e4m3(value(c) / scale);
+    }
+  }
+}
+
+// dw[c] = sum over the G partial rows in a fixed order, cast to W.  One CTA of 32 warps per
+// 32 columns: warp w sums partial rows w, w+32, ..., the warp sums are added in warp order.
+template <typename W>
+__global__ void __launch_bounds__(1024) add_rmsnorm_dw_reduce(const float* __restrict__ part,
+                                                              int G, int64_t cols,
+                                                              W* __restrict__ dw) {
+  __shared__ float red[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (c < cols) {
+#pragma unroll 8
+    for (int g = warp; g < G; g += 32) s += part[(int64_t)g * cols + c];
+  }
+  red[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && c < cols) {
+    float t = 0.f;
+    for (int i = 0; i < 32; ++i) t += red[i][lane];
+    dw[c] = Elt<W>::from_f(t);
+  }
+}
+
+constexpr int kMaxGridPerSm = 8;
+inline int row_grid(int64_t rows) {
+  const int64_t g = (int64_t)num_sms() * kMaxGridPerSm;
+  return (int)(rows < g ? rows : g);
+}
+inline size_t bwd_ws_bytes(int64_t rows, int64_t cols) {
+  return (size_t)row_grid(rows) * (size_t)cols * sizeof(float);
+}
+
+template <typename T, typename R>
+int fwd_t(const void* x, int64_t xs, const void* r, int64_t rs, const void* w, int wd, void* y,
+          void* h, float* rstd, int64_t rows, int64_t cols, float eps, cudaStream_t st) {
+  add_rmsnorm_fwd_generic<T, R><<<row_grid(rows), 256, 0, st>>>(
+      static_cast<const T*>(x), xs, static_cast<const R*>(r), rs, w, wd, static_cast<T*>(y),
+      static_cast<R*>(h), rstd, rows, cols, eps);
+  return launch_status("fk_add_rmsnorm_fwd");
+}
+
+template <typename T, typename R>
+int bwd_t(const void* dy, int64_t dys, const void* dh, int64_t dhs, const void* h, const void* w,
+          int wd, const float* rstd, void* dx, void* dr, float* part, int64_t rows, int64_t cols,
+          int* grid, cudaStream_t st) {
+  *grid = row_grid(rows);
+  add_rmsnorm_bwd_generic<T, R><<<*grid, 256, 0, st>>>(
+      static_cast<const T*>(dy), dys, static_cast<const R*>(dh), dhs, static_cast<const R*>(h), w,
+      wd, rstd, static_cast<T*>(dx), static_cast<R*>(dr), part, rows, cols);
+  return launch_status("fk_add_rmsnorm_bwd");
+}
+
+template <typename T, typename R>
+int quant_t(const void* x, int64_t xs, const void* r, int64_t rs, const void* w, int wd, void* q,
+            float* scales, void* h, int64_t rows, int64_t cols, int64_t block, float eps,
+            cudaStream_t st) {
+  add_rmsnorm_quant_generic<T, R><<<row_grid(rows), 256, 0, st>>>(
+      static_cast<const T*>(x), xs, static_cast<const R*>(r), rs, w, wd,
+      static_cast<uint8_t*>(q), scales, static_cast<R*>(h), rows, cols, block, eps);
+  return launch_status("fk_add_rmsnorm_quant");
+}
+
+}  // namespace
+}  // namespace fk
+
+// Binds T (dtype) and R (the residual's type: dtype or FK_F32).
+#define FK_DISPATCH_TR(dtype, r_dtype, ...)                                  \
+  FK_DISPATCH_DTYPE(dtype, {                                                 \
+    if ((r_dtype) == (dtype)) { using res_t = scalar_t; __VA_ARGS__; }       \
+    else { using res_t = float; __VA_ARGS__; }                               \
+  })
+
+extern "C" int fk_add_rmsnorm_fwd(const void* x, int64_t x_row_stride, const void* r,
+                                  int64_t r_row_stride, int r_dtype, const void* weight,
+                                  int w_dtype, void* y, void* h, float* rstd, int64_t rows,
+                                  int64_t cols, float eps, int dtype, void* stream) {
+  FK_CHECK_ARG(rows >= 0 && cols >= 1, "fk_add_rmsnorm_fwd: bad shape [%lld, %lld]",
+               (long long)rows, (long long)cols);
+  FK_CHECK_ARG(fk::valid_dtype(dtype) && fk::valid_dtype(w_dtype), "fk_add_rmsnorm_fwd: bad dtype");
+  FK_CHECK_ARG(r_dtype == dtype || r_dtype == FK_F32,
+               "fk_add_rmsnorm_fwd: the residual has x's type or fp32");
+  FK_CHECK_ARG(x_row_stride >= cols && r_row_stride >= cols,
+               "fk_add_rmsnorm_fwd: row stride < cols");
+  if (rows == 0) return FK_OK;
+  FK_CHECK_ARG(x && r && weight && y && h, "fk_add_rmsnorm_fwd: null pointer");
+  FK_DISPATCH_TR(dtype, r_dtype, return (fk::fwd_t<scalar_t, res_t>(
+                                     x, x_row_stride, r, r_row_stride, weight, w_dtype, y, h, rstd,
+                                     rows, cols, eps, fk::as_stream(stream))));
+  return FK_OK;
+}
+
+extern "C" int fk_add_rmsnorm_bwd_workspace_size(int64_t rows, int64_t cols, size_t* bytes) {
+  FK_CHECK_ARG(bytes != nullptr, "fk_add_rmsnorm_bwd_workspace_size: null output");
+  FK_CHECK_ARG(rows >= 0 && cols >= 1, "fk_add_rmsnorm_bwd_workspace_size: bad shape");
+  *bytes = rows == 0 ? 0 : fk::bwd_ws_bytes(rows, cols);
+  return FK_OK;
+}
+
+extern "C" int fk_add_rmsnorm_bwd(const void* dy, int64_t dy_row_stride, const void* dh,
+                                  int64_t dh_row_stride, const void* h, int r_dtype,
+                                  const void* weight, int w_dtype, const float* rstd, void* dx,
+                                  void* dr, void* dw, void* workspace, size_t workspace_bytes,
+                                  int64_t rows, int64_t cols, int dtype, void* stream) {
+  FK_CHECK_ARG(rows >= 0 && cols >= 1, "fk_add_rmsnorm_bwd: bad shape [%lld, %lld]",
+               (long long)rows, (long long)cols);
+  FK_CHECK_ARG(fk::valid_dtype(dtype) && fk::valid_dtype(w_dtype), "fk_add_rmsnorm_bwd: bad dtype");
+  FK_CHECK_ARG(r_dtype == dtype || r_dtype == FK_F32,
+               "fk_add_rmsnorm_bwd: the residual has x's type or fp32");
+  FK_CHECK_ARG(dw && weight, "fk_add_rmsnorm_bwd: null pointer");
+  cudaStream_t st = fk::as_stream(stream);
+  if (rows == 0) {
+    cudaMemsetAsync(dw, 0, (size_t)cols * fk::dtype_size(w_dtype), st);
+    return fk::launch_status("fk_add_rmsnorm_bwd(zero dw)");
+  }
+  FK_CHECK_ARG(dy && h && rstd && dx, "fk_add_rmsnorm_bwd: null pointer");
+  FK_CHECK_ARG(dr || r_dtype == dtype, "fk_add_rmsnorm_bwd: dr is needed where the types differ");
+  FK_CHECK_ARG(dy_row_stride >= cols && (!dh || dh_row_stride >= cols),
+               "fk_add_rmsnorm_bwd: row stride < cols");
+  const size_t need = fk::bwd_ws_bytes(rows, cols);
+  if (workspace == nullptr || workspace_bytes < need || !fk::aligned16(workspace))
+    return fk::fail(FK_ERR_WORKSPACE,
+                    "fk_add_rmsnorm_bwd: need %zu aligned workspace bytes, got %zu", need,
+                    workspace_bytes);
+  float* part = static_cast<float*>(workspace);
+  int grid = 0, s = FK_OK;
+  FK_DISPATCH_TR(dtype, r_dtype, s = (fk::bwd_t<scalar_t, res_t>(
+                                     dy, dy_row_stride, dh, dh_row_stride, h, weight, w_dtype,
+                                     rstd, dx, r_dtype == dtype ? nullptr : dr, part, rows, cols,
+                                     &grid, st)));
+  if (s != FK_OK) return s;
+  const unsigned rgrid = (unsigned)((cols + 31) / 32);
+  FK_DISPATCH_DTYPE(w_dtype, (fk::add_rmsnorm_dw_reduce<scalar_t><<<rgrid, 1024, 0, st>>>(
+                                 part, grid, cols, static_cast<scalar_t*>(dw))));
+  return fk::launch_status("fk_add_rmsnorm_bwd(dw reduce)");
+}
+
+extern "C" int fk_add_rmsnorm_quant(const void* x, int64_t x_row_stride, const void* r,
+                                    int64_t r_row_stride, int r_dtype, const void* weight,
+                                    int w_dtype, void* q, float* scales, void* h, int64_t rows,
+                                    int64_t cols, int64_t block, float eps, int dtype,
+                                    void* stream) {
+  FK_CHECK_ARG(rows >= 0 && cols >= 1, "fk_add_rmsnorm_quant: bad shape [%lld, %lld]",
+               (long long)rows, (long long)cols);
+  FK_CHECK_ARG(fk::valid_dtype(dtype) && fk::valid_dtype(w_dtype),
+               "fk_add_rmsnorm_quant: bad dtype");
+  FK_CHECK_ARG(r_dtype == dtype || r_dtype == FK_F32,
+               "fk_add_rmsnorm_quant: the residual has x's type or fp32");
+  FK_CHECK_ARG(block == 0 || block == 128, "fk_add_rmsnorm_quant: block is 0 (the row) or 128");
+  FK_CHECK_ARG(x_row_stride >= cols && (!r || r_row_stride >= cols),
+               "fk_add_rmsnorm_quant: row stride < cols");
+  if (rows == 0) return FK_OK;
+  FK_CHECK_ARG(x && weight && q && scales, "fk_add_rmsnorm_quant: null pointer");
+  FK_CHECK_ARG(!r || h, "fk_add_rmsnorm_quant: h is needed with a residual");
+  FK_DISPATCH_TR(dtype, r_dtype, return (fk::quant_t<scalar_t, res_t>(
+                                     x, x_row_stride, r, r_row_stride, weight, w_dtype, q, scales,
+                                     h, rows, cols, block ? block : cols, eps,
+                                     fk::as_stream(stream))));
+  return FK_OK;
+}

@@ -9,6 +9,7 @@ device in a fixed order (per-CTA partial rows + a column reduce), replacing the
 """
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -58,3 +59,135 @@ class FusedRMSNorm(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return _FusedRMSNormFn.apply(x, self.weight, self.eps)
+
+
+# ---------------------------------------------------------------- with the residual's addition
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _check_add_norm(x, residual, weight):
+    assert x.is_cuda and weight.is_cuda and x.ndim >= 1
+    assert x.dtype in _FLOATS and weight.dtype in _FLOATS, "fp32, fp16 or bf16 tensors"
+    assert weight.numel() == x.shape[-1] and x.shape[-1] >= 1
+    assert weight.device == x.device
+    if residual is not None:
+        assert residual.shape == x.shape, "residual and x have one shape (nothing is broadcast)"
+        assert residual.device == x.device
+        assert residual.dtype in (x.dtype, torch.float32), "the residual has x's dtype or fp32"
+
+
+class _FusedAddRMSNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, save):
+        ctx.set_materialize_grads(False)
+        n_cols = x.shape[-1]
+        x2, r2 = _lib.rows_of(x, n_cols), _lib.rows_of(residual, n_cols)
+        n_rows = x2.shape[0]
+        w = weight.contiguous()
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+        rstd = torch.empty(n_rows, dtype=torch.float32, device=x.device) if save else None
+        with _lib.on_device(x):
+            _lib.call("fk_add_rmsnorm_fwd", x2.data_ptr(), _lib.row_stride(x2), r2.data_ptr(),
+                      _lib.row_stride(r2), _lib.dtype_code(r2.dtype), w.data_ptr(),
+                      _lib.dtype_code(w.dtype), y.data_ptr(), h.data_ptr(), _lib.ptr(rstd),
+                      n_rows, n_cols, float(eps), _lib.dtype_code(x2.dtype), _lib.stream_of(x))
+        if save:
+            ctx.save_for_backward(h, w, rstd)
+            ctx.x_dtype = x.dtype
+            ctx.weight_shape = weight.shape
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        h, w, rstd = ctx.saved_tensors
+        shape, n_cols = h.shape, h.shape[-1]
+        need_x, need_r, need_w = ctx.needs_input_grad[:3]
+        if dy is None:  # only the sum was used: its gradient passes through
+            if dh is None:
+                return None, None, None, None, None
+            return (dh.to(ctx.x_dtype) if need_x else None, dh if need_r else None,
+                    torch.zeros(ctx.weight_shape, dtype=w.dtype, device=w.device)
+                    if need_w else None, None, None)
+        dy2 = _lib.rows_of(dy, n_cols)
+        dh2 = None if dh is None else _lib.rows_of(dh, n_cols)
+        n_rows = dy2.shape[0]
+        dx = torch.empty(shape, dtype=ctx.x_dtype, device=h.device)
+        dr = dx if h.dtype == ctx.x_dtype else torch.empty_like(h)
+        dw = torch.empty(ctx.weight_shape, dtype=w.dtype, device=h.device)
+        ws = torch.empty(max(_lib.workspace_bytes("fk_add_rmsnorm_bwd_workspace_size", h.device,
+                                                  n_rows, n_cols), 16),
+                         dtype=torch.uint8, device=h.device)
+        with _lib.on_device(h):
+            _lib.call("fk_add_rmsnorm_bwd", dy2.data_ptr(), _lib.row_stride(dy2), _lib.ptr(dh2),
+                      0 if dh2 is None else _lib.row_stride(dh2), h.data_ptr(),
+                      _lib.dtype_code(h.dtype), w.data_ptr(), _lib.dtype_code(w.dtype),
+                      rstd.data_ptr(), dx.data_ptr(), None if dr is dx else dr.data_ptr(),
+                      dw.data_ptr(), ws.data_ptr(), ws.numel(), n_rows, n_cols,
+                      _lib.dtype_code(ctx.x_dtype), _lib.stream_of(h))
+        return dx if need_x else None, dr if need_r else None, dw if need_w else None, None, None
+
+
+def fused_add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                       eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """``h = x + residual`` and ``y = h * rsqrt(mean(h^2) + eps) * weight`` in one pass over
+    the last dimension; returns ``(y, h)``, ``y`` in x's dtype and ``h`` in the residual's
+    (x's dtype, or fp32 for a residual stream kept in 32 bits).
+
+    The norm is that of the rounded ``h``, so the result is that of the addition followed by
+    ``FusedRMSNorm``; in the backward pass the gradient that arrives at ``h`` is added in 32
+    bits before the one rounding of the inputs' gradient."""
+    _check_add_norm(x, residual, weight)
+    save = torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or
+                                        weight.requires_grad)
+    return _FusedAddRMSNormFn.apply(x, residual, weight, eps, save)
+
+
+def fused_add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None,
+                             weight: torch.Tensor, eps: float = 1e-6, block: int | None = None
+                             ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """RMSNorm of ``h = x + residual`` (of ``x`` itself where residual is None) with its
+    output in 8 bits: returns ``(q, scales, h)``, ``q`` float8_e4m3fn of x's shape with
+    ``y ~ q * scales``.
+
+    ``block=None`` gives one fp32 scale per row (scales [..., 1]), ``block=128`` one per 128
+    columns (scales [..., ceil(cols / 128)]): max|y| / 448 over the group, at least 2^-126.  The
+    32-bit ``y`` is quantised, so it is rounded once.  It is a forward for inference and for the
+    8-bit side of a product: it has no gradient, and asserts that none is asked for."""
+    _check_add_norm(x, residual, weight)
+    assert block in (None, 128), "block is None (a scale per row) or 128"
+    assert not (torch.is_grad_enabled() and
+                (x.requires_grad or weight.requires_grad or
+                 (residual is not None and residual.requires_grad))), \
+        "fused_add_rms_norm_quant has no gradient: call it under torch.no_grad()"
+    n_cols = x.shape[-1]
+    x2 = _lib.rows_of(x, n_cols)
+    n_rows = x2.shape[0]
+    w = weight.contiguous()
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    groups = 1 if block is None else -(-n_cols // block)
+    scales = torch.empty(*x.shape[:-1], groups, dtype=torch.float32, device=x.device)
+    r2, h = None, x
+    if residual is not None:
+        r2 = _lib.rows_of(residual, n_cols)
+        h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+    with _lib.on_device(x):
+        _lib.call("fk_add_rmsnorm_quant", x2.data_ptr(), _lib.row_stride(x2), _lib.ptr(r2),
+                  0 if r2 is None else _lib.row_stride(r2),
+                  _lib.dtype_code(x2.dtype if r2 is None else r2.dtype), w.data_ptr(),
+                  _lib.dtype_code(w.dtype), q.data_ptr(), scales.data_ptr(),
+                  None if r2 is None else h.data_ptr(), n_rows, n_cols, block or 0, float(eps),
+                  _lib.dtype_code(x2.dtype), _lib.stream_of(x))
+    return q, scales, h
+
+
+class FusedAddRMSNorm(FusedRMSNorm):
+    """``FusedRMSNorm`` that takes the residual stream along: ``forward(x, residual)`` returns
+    ``(norm(x + residual), x + residual)``; with residual None, ``(norm(x), x)``.  Same
+    parameter and state_dict key."""
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        if residual is None:
+            return super().forward(x), x
+        return fused_add_rms_norm(x, residual, self.weight, self.eps)

@@ -105,6 +105,38 @@ FK_API int fk_rmsnorm_bwd_noalloc(const void* dy, const void* x, const void* wei
                                   const float* rstd, void* dx, void* dw, int64_t rows,
                                   int64_t cols, int dtype, void* stream);
 
+/* ---------------------------------------------------------------- add + RMSNorm --
+ * No counterpart in the reference (its blocks add and normalise in separate passes).
+ * h = x + r rounded to r_dtype (x's type, or FK_F32 for a residual stream in 32 bits);
+ * y = h * rsqrt(mean(h^2) + eps) * w in x's type, of the rounded h; rstd[row] is kept for
+ * the backward (NULL: not wanted).  x and r have row strides, y and h are contiguous. */
+FK_API int fk_add_rmsnorm_fwd(const void* x, int64_t x_row_stride, const void* r,
+                              int64_t r_row_stride, int r_dtype, const void* weight, int w_dtype,
+                              void* y, void* h, float* rstd, int64_t rows, int64_t cols,
+                              float eps, int dtype, void* stream);
+
+/* Bytes of workspace fk_add_rmsnorm_bwd needs for this shape on the current device. */
+FK_API int fk_add_rmsnorm_bwd_workspace_size(int64_t rows, int64_t cols, size_t* bytes);
+
+/* g = dh + rstd*w*dy - h*rstd^3*mean(w*dy*h) (dh NULL: 0), added in fp32 and rounded to
+ * dx (dtype) and dr (r_dtype; only where the types differ, else dx serves both inputs);
+ * dw = sum_rows(dy*h*rstd), fixed-order sums.  dy (dtype) and dh (r_dtype) have row
+ * strides, the other tensors are contiguous. */
+FK_API int fk_add_rmsnorm_bwd(const void* dy, int64_t dy_row_stride, const void* dh,
+                              int64_t dh_row_stride, const void* h, int r_dtype,
+                              const void* weight, int w_dtype, const float* rstd, void* dx,
+                              void* dr, void* dw, void* workspace, size_t workspace_bytes,
+                              int64_t rows, int64_t cols, int dtype, void* stream);
+
+/* The forward with y in 8 bits: per group of `block` columns (0: the row; or 128, the last
+ * group of a row may be short) scale = max(max|y| / 448, 2^-126) and q = e4m3(y / scale),
+ * saturating, with y in fp32.  scales: [rows, ceil(cols / block)].  r and h may be NULL
+ * (h is x then). */
+FK_API int fk_add_rmsnorm_quant(const void* x, int64_t x_row_stride, const void* r,
+                                int64_t r_row_stride, int r_dtype, const void* weight,
+                                int w_dtype, void* q, float* scales, void* h, int64_t rows,
+                                int64_t cols, int64_t block, float eps, int dtype, void* stream);
+
 /* ---------------------------------------------------------------- MoE router -----
  * Per row of logits [n_rows, n_experts] (row stride in elements): rank experts by the
  * exact logit value (ties -> lower expert index first; -0.0 == +0.0; NaN ranks above
@@ -145,6 +177,47 @@ FK_API int fk_ce_fwd(const void* logits, int64_t row_stride, void* grad, int64_t
  * Replaces the `grad * scale` of cross_entropy.py:115-116. */
 FK_API int fk_ce_bwd_scale(void* grad, int64_t grad_row_stride, int64_t n_rows, int64_t n_cols,
                     const float* grad_output, int dtype, void* stream);
+
+/* ---------------------------------------------------------------- distillation ---
+ * No counterpart in the reference.  Loss and gradient of logits [n_rows, n_cols] against a
+ * teacher's top logits (teacher_idx, teacher_logits: [n_rows, k], k <= 1024, id < 0 =
+ * unused slot) and, with targets, the hard labels:
+ *   p = softmax(teacher / T) over the used slots,  q = softmax(row / T),
+ *   row loss = (1-a) T^2 sum_j p_j (log p_j - log q[id_j]) + a (logsumexp(row) - x_target),
+ *   gradient = loss_scale/n * [(1-a) T (q - P) + a (softmax(row) - onehot)],
+ * a = hard_weight (0 without targets), P_c = sum of the p_j with id c.  Counted rows (n, at
+ * least 1): target != ignore_index, or without targets those that hold a teacher; the others
+ * get loss 0 and a zero gradient row.  A row whose slots are all unused or -inf has no soft
+ * part.  An id or target out of range sets *err_flag = 1 and makes that row's loss and
+ * gradient NaN.  loss[0] is the mean over the counted rows (fixed-order sum), not scaled by
+ * loss_scale.  grad may be NULL (loss only) or alias logits.  The gradient is for
+ * grad_output == loss_scale; fk_ce_bwd_scale turns it into another one. */
+FK_API int fk_distill_workspace_size(int64_t n_rows, int k, size_t* bytes);
+FK_API int fk_distill(const void* logits, int64_t row_stride, void* grad,
+                      int64_t grad_row_stride, const int64_t* teacher_idx,
+                      const void* teacher_logits, int teacher_dtype, int k,
+                      const int64_t* targets, int64_t n_rows, int64_t n_cols,
+                      int64_t ignore_index, float temperature, float hard_weight,
+                      float loss_scale, int dtype, float* loss, int* err_flag, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- MoE balance loss
+ * No counterpart in the reference.  For the router's logits [n_rows, n_experts] (row stride
+ * in elements, n_experts <= 256) and its choices idx [n_rows, k], over the tokens whose
+ * token_mask byte is not 0 (NULL: all of them), n of them (at least 1):
+ *   counts[e] = slots that name e,  f = counts / max(1, sum of counts),  p = softmax(row),
+ *   S = sum_e f_e p_e,  loss = E/n sum S + z_coef/n sum lse^2,
+ *   grad = loss_scale * p_e * (E/n (f_e - S) + 2 z_coef/n lse).
+ * A negative idx is an unused slot; one >= n_experts makes loss and gradient NaN.  Masked
+ * tokens get a zero gradient row.  grad [n_rows, n_experts] is contiguous, in the logits'
+ * type (NULL: not wanted); loss is not scaled by loss_scale.  Integer counts and
+ * fixed-order sums: the results do not depend on the order in which CTAs run. */
+FK_API int fk_moe_balance_workspace_size(size_t* bytes);
+FK_API int fk_moe_balance(const void* logits, int64_t row_stride, const int64_t* idx,
+                          const uint8_t* token_mask, int64_t n_rows, int n_experts, int k,
+                          float z_coef, float loss_scale, void* grad, int64_t* counts,
+                          float* loss, void* workspace, size_t workspace_bytes, int dtype,
+                          void* stream);
 
 /* ---------------------------------------------------------------- MoE sorted dispatch
  * Sorted-row layout: the n_tokens*k (token, slot) assignments are laid out expert-major,

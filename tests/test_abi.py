@@ -89,3 +89,75 @@ def test_ep_planning_workspace_and_peer_argument_checks():
     assert lib.fk_ep_peer_wait(None, 0, 0, None, 100, None, None) == 1
     assert lib.fk_ipc_alloc(0, None, None) == 1
     assert lib.fk_ipc_open(None, None) == 1
+
+
+def test_add_rmsnorm_argument_checks():
+    """Refused on the host, before any device work."""
+    lib = _lib.load()
+    F32, F16, BF16 = 0, 1, 2
+
+    def fwd(xs=8, rs=8, rd=BF16, wd=F32, rows=4, cols=8, dt=BF16):
+        return lib.fk_add_rmsnorm_fwd(None, xs, None, rs, rd, None, wd, None, None, None, rows, cols,
+                                      1e-6, dt, None)
+
+    assert fwd() == 1 and b"null" in lib.fk_last_error()
+    assert fwd(rows=0) == 0
+    assert fwd(rows=-1) == 1 and fwd(cols=0) == 1 and fwd(xs=7) == 1 and fwd(rs=7) == 1
+    assert fwd(rd=F16) == 1 and fwd(dt=7) == 1 and fwd(wd=7) == 1
+    assert fwd(dt=F32, rd=BF16) == 1  # a residual narrower than x
+    n = ctypes.c_size_t(0)
+    assert lib.fk_add_rmsnorm_bwd_workspace_size(10, 8, None) == 1
+    assert lib.fk_add_rmsnorm_bwd_workspace_size(10, 0, ctypes.byref(n)) == 1
+    assert lib.fk_add_rmsnorm_bwd_workspace_size(10, 8, ctypes.byref(n)) == 0 and n.value > 0
+
+    def bwd(ptr=1, dr=None, ws=None, size=0, rd=BF16, stride=8):
+        return lib.fk_add_rmsnorm_bwd(ptr, stride, None, 0, ptr, rd, ptr, F32, ptr, ptr, dr, ptr, ws,
+                                      size, 4, 8, BF16, None)
+
+    assert bwd(ptr=None) == 1 and bwd(rd=F32) == 1 and bwd(stride=7) == 1
+    assert bwd() == 4 and bwd(ws=8, size=1 << 30) == 4  # no workspace; one off its alignment
+
+    def quant(block=0, r=None, h=None, rows=4):
+        return lib.fk_add_rmsnorm_quant(1, 8, r, 8, BF16, 1, F32, 1, 1, h, rows, 8, block, 1e-6, BF16,
+                                        None)
+
+    assert quant(block=64) == 1 and quant(block=-1) == 1 and quant(r=1) == 1
+    assert quant(rows=0) == 0
+
+
+def test_balance_argument_checks():
+    lib = _lib.load()
+    n = ctypes.c_size_t(0)
+    assert lib.fk_moe_balance_workspace_size(None) == 1
+    assert lib.fk_moe_balance_workspace_size(ctypes.byref(n)) == 0 and n.value > 0
+
+    def run(stride=8, rows=4, e=8, k=2, dt=0, ptr=16, ws=16, size=1 << 30):
+        return lib.fk_moe_balance(ptr, stride, ptr, None, rows, e, k, 0.0, 1.0, None, ptr, ptr, ws,
+                                  size, dt, None)
+
+    assert run(e=257, stride=257) == 2 and b"257" in lib.fk_last_error()
+    assert run(rows=-1) == 1 and run(e=0) == 1 and run(stride=7) == 1 and run(dt=3) == 1
+    assert run(rows=1 << 30, k=2) == 1  # slots are counted in 32 bits
+    assert run(ptr=None) == 1
+    assert run(ws=None) == 4 and run(ws=8) == 4 and run(size=16) == 4
+
+
+def test_distill_argument_checks():
+    lib = _lib.load()
+    n = ctypes.c_size_t(0)
+    assert lib.fk_distill_workspace_size(4, 2, None) == 1
+    assert lib.fk_distill_workspace_size(4, 0, ctypes.byref(n)) == 1
+    assert lib.fk_distill_workspace_size(4, 2, ctypes.byref(n)) == 0 and n.value > 0
+
+    def run(ptr=16, stride=8, grad=None, gstride=0, k=2, rows=4, cols=8, t=1.0, hw=0.5, dt=0, tdt=0,
+            ws=16, size=1 << 30):
+        return lib.fk_distill(ptr, stride, grad, gstride, ptr, ptr, tdt, k, None, rows, cols, -100, t,
+                              hw, 1.0, dt, ptr, ptr, ws, size, None)
+
+    assert run(k=1025) == 2 and b"1025" in lib.fk_last_error()
+    assert run(k=0) == 1 and run(rows=-1) == 1 and run(cols=0) == 1 and run(stride=7) == 1
+    assert run(cols=1 << 31, stride=1 << 31) == 1 and run(grad=16, gstride=7) == 1
+    assert run(t=0.0) == 1 and run(t=float("inf")) == 1 and run(t=float("nan")) == 1
+    assert run(hw=1.5) == 1 and run(hw=float("nan")) == 1 and run(dt=3) == 1 and run(tdt=-1) == 1
+    assert run(ptr=None) == 1
+    assert run(ws=None) == 4 and run(ws=8) == 4 and run(size=16) == 4
