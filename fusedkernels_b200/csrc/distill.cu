@@ -13,6 +13,7 @@
 // for the two sums and once for its gradient, and the gradient at the listed ids is computed
 // from the logit itself, in 32 bits, and rounded once.
 #include "common.cuh"
+#include "ptx.cuh"
 
 namespace fk {
 namespace {
@@ -20,15 +21,14 @@ namespace {
 constexpr int kMaxSlots = 1024;
 constexpr int kTeacherWarps = 8;
 constexpr int kTeacherCtas = 64;   // partial counts that every CTA of the second kernel adds up
-constexpr int kRowThreads = 256;
-constexpr int kRowCtasPerSm = 4;
+constexpr int kMaxRowCtasPerSm = 16;
 // Row states.
 constexpr int kSkip = 0, kSoft = 1, kHard = 2, kBad = 4;
 
 struct Workspace {
   int2* valid;       // [kTeacherCtas] (rows that count, rows with an id out of range)
   unsigned* ticket;
-  float* loss_rows;  // [n_rows]
+  double* sums;      // [kMaxRowCtasPerSm * SMs]  loss of the rows of one CTA
   float* entropy;    // [n_rows]  sum p log p
   int* state;        // [n_rows]
   int* ids;          // [n_rows][list]  -1 = empty
@@ -46,7 +46,7 @@ inline size_t ws_layout(void* base, int64_t n_rows, int k, Workspace* w) {
   const size_t n = (size_t)n_rows, list = (size_t)k + 1;
   w->valid = reinterpret_cast<int2*>(take(kTeacherCtas * 8));
   w->ticket = reinterpret_cast<unsigned*>(take(4));
-  w->loss_rows = reinterpret_cast<float*>(take(n * 4));
+  w->sums = reinterpret_cast<double*>(take((size_t)num_sms() * kMaxRowCtasPerSm * 8));
   w->entropy = reinterpret_cast<float*>(take(n * 4));
   w->state = reinterpret_cast<int*>(take(n * 4));
   w->ids = reinterpret_cast<int*>(take(n * list * 4));
@@ -198,7 +198,7 @@ struct RowArgs {
   const int* state;
   const int* ids;
   const float* probs;
-  float* loss_rows;
+  double* sums;
   unsigned* ticket;
   float* loss;
   int* err;
@@ -208,19 +208,21 @@ struct RowArgs {
   float temperature, inv_t, hard_weight, loss_scale;
 };
 
-// Rows that count, at least 1 (all threads return the same number).
+// Rows that count, at least 1 (whole warps call; all threads return the same number).
 __device__ __forceinline__ float count_valid(const RowArgs& a) {
   int n = 0;
-  for (int i = 0; i < a.teacher_ctas; ++i) n += a.valid[i].x;
+  for (int i = threadIdx.x & 31; i < a.teacher_ctas; i += 32) n += a.valid[i].x;
+  n = __reduce_add_sync(0xffffffffu, n);
   return (float)(n < 1 ? 1 : n);
 }
 
-// The CTA that ends last adds the row losses up in a fixed order.
-__device__ __forceinline__ void finish_loss(const RowArgs& a, float n) {
+// Thread 0 leaves the loss of its CTA's rows; the CTA that ends last adds them up in a fixed
+// order (at most 16 per SM).
+__device__ __forceinline__ void finish_loss(const RowArgs& a, float n, double mine) {
   __shared__ bool last;
   __shared__ double red[32];
-  __syncthreads();
   if (threadIdx.x == 0) {
+    a.sums[blockIdx.x] = mine;
     __threadfence();
     last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
   }
@@ -228,7 +230,7 @@ __device__ __forceinline__ void finish_loss(const RowArgs& a, float n) {
   if (!last) return;
   __threadfence();
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < a.n_rows; i += blockDim.x) s += (double)__ldcg(a.loss_rows + i);
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += blockDim.x) s += __ldcg(a.sums + i);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
@@ -243,21 +245,25 @@ __device__ __forceinline__ void finish_loss(const RowArgs& a, float n) {
   }
 }
 
-// One CTA per row, element loops (any stride and alignment).
+// ------------------------------------------------------------------ rows, any layout ----
+constexpr int kGenericThreads = 256;
+
+// One CTA per row, element loops (any stride, alignment and length).
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) distill_rows_generic(
+__global__ void __launch_bounds__(kGenericThreads) distill_rows_generic(
     const T* logits, int64_t lstride, T* grad, int64_t gstride, RowArgs a) {
   __shared__ float red[32];
   __shared__ float picked[kMaxSlots + 1];
   const float n = count_valid(a);
   const bool two = a.temperature != 1.0f;
+  double total = 0.0;
   for (int64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x) {
     const T* src = logits + row * lstride;
     T* dst = grad ? grad + row * gstride : nullptr;
     const int state = a.state[row];
     if (state == kSkip || state == kBad) {
       const float z = state == kBad ? __int_as_float(0x7fc00000) : 0.f;
-      if (threadIdx.x == 0) a.loss_rows[row] = z;
+      total += (double)z;
       if (dst)
         for (int c = threadIdx.x; c < a.n_cols; c += blockDim.x) dst[c] = Elt<T>::from_f(z);
       continue;
@@ -290,16 +296,14 @@ __global__ void __launch_bounds__(kRowThreads) distill_rows_generic(
       if (sw > 0.f)
         l = sw * a.temperature * a.temperature * (a.entropy[row] - dot * a.inv_t + logf(zt));
       if (hw > 0.f) l += hw * (logf(z1) - picked[a.list - 1]);
-      a.loss_rows[row] = l;
+      total += (double)l;
     }
     if (dst) {
       const float ct = sw * a.temperature * a.loss_scale / n, c1 = hw * a.loss_scale / n;
       const float kt = ct / zt, k1 = c1 / z1;
       auto dense = [&](float d) {
-        float g = kt * expf(d * a.inv_t);
-        if (two) g = fmaf(k1, expf(d), g);
-        else g = fmaf(k1, expf(d * a.inv_t), g);
-        return g;
+        const float e = expf(d * a.inv_t);
+        return fmaf(kt, e, k1 * (two ? expf(d) : e));
       };
       for (int c = threadIdx.x; c < a.n_cols; c += blockDim.x)
         dst[c] = Elt<T>::from_f(dense(Elt<T>::to_f(src[c]) - base));
@@ -313,16 +317,475 @@ __global__ void __launch_bounds__(kRowThreads) distill_rows_generic(
     }
     __syncthreads();  // picked is the next row's from here
   }
-  finish_loss(a, n);
+  finish_loss(a, n, total);
+}
+
+// ------------------------------------------------------------------ rows, 16-byte packets
+// A cluster of 1, 2, 4 or 8 CTAs takes a row; each CTA has a slice of its 16-byte packets, at
+// most KP per thread.  Slices arrive through a ring of kStages shared-memory buffers filled by
+// cp.async.bulk, so the next rows are on their way while a row is worked on; a slice then lies
+// in registers, and its buffer is refilled as soon as every thread has taken its packets.
+//
+// Each logit is exponentiated once: e = exp((x - m_t) / T) with the thread's own maximum m_t
+// stays in registers, and after the row's maximum m and sum z are known the gradient is
+// e * [exp((m_t - m) / T) * k / z].  (With two temperatures and 16-bit logits the registers do
+// not hold both exponentials, and they are formed again from the logits.)  The CTAs of a row
+// exchange (m, z) by st.async into each other's shared memory.
+//
+// Elements before the first and after the last 16-byte boundary of a row (any odd width or
+// offset) are taken singly by the first CTA.  Logits and gradient have to have the same
+// offset from a 16-byte boundary in every row; other layouts take the generic kernel.
+constexpr int kStages = 3;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// exp(d) of a scaled difference d <= 0: 16-bit gradients round to 8 or 11 bits, so one ex2 is
+// exact enough; 32-bit ones take expf.
+template <typename T>
+__device__ __forceinline__ float exp_of(float d) { return ex2f(d * kLog2e); }
+template <>
+__device__ __forceinline__ float exp_of<float>(float d) { return expf(d); }
+
+// exp of a pair.  16 bits: as above.  32 bits: 2^(d log2 e) with the product in two parts,
+// hi + lo (log2 e = kLog2e + kLog2eLow, the roundings of the products caught by FMAs), so that
+// the error stays that of ex2 (2 ulp) for any d: 2^hi * (1 + lo ln 2), lo being below 2^-16.
+// d is held at -200 from below (2^hi is 0 there), so that -inf does not meet its own residual.
+constexpr float kLog2eLow = 1.9259629911266174e-8f;
+constexpr float kLn2 = 0.69314718055994531f;
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 exp2_of(float2 d) {
+  d = make_float2(max_or_nan(d.x, -200.f), max_or_nan(d.y, -200.f));
+  const float2 hi = __fmul2_rn(d, make_float2(kLog2e, kLog2e));
+  float2 lo = __ffma2_rn(d, make_float2(kLog2e, kLog2e), make_float2(-hi.x, -hi.y));
+  lo = __ffma2_rn(d, make_float2(kLog2eLow, kLog2eLow), lo);
+  const float2 p = make_float2(ex2f(hi.x), ex2f(hi.y));
+  return __ffma2_rn(__fmul2_rn(p, make_float2(kLn2, kLn2)), lo, p);
+}
+
+template <typename T> struct Pair;  // two neighbouring elements
+template <> struct Pair<__nv_bfloat16> {
+  static constexpr uint32_t kNegInf = 0xff80ff80u;
+  __nv_bfloat162 v;
+  __device__ __forceinline__ float2 f() const { return __bfloat1622float2(v); }
+  __device__ __forceinline__ void set(float2 a) { v = __float22bfloat162_rn(a); }
+  __device__ __forceinline__ void take_max(const Pair& b) { v = __hmax2(v, b.v); }
+};
+template <> struct Pair<__half> {
+  static constexpr uint32_t kNegInf = 0xfc00fc00u;
+  __half2 v;
+  __device__ __forceinline__ float2 f() const { return __half22float2(v); }
+  __device__ __forceinline__ void set(float2 a) { v = __float22half2_rn(a); }
+  __device__ __forceinline__ void take_max(const Pair& b) { v = __hmax2(v, b.v); }
+};
+template <> struct Pair<float> {
+  static constexpr uint32_t kNegInf = 0xff800000u;
+  float2 v;
+  __device__ __forceinline__ float2 f() const { return v; }
+  __device__ __forceinline__ void set(float2 a) { v = a; }
+  __device__ __forceinline__ void take_max(const Pair& b) {
+    v = make_float2(fmaxf(v.x, b.v.x), fmaxf(v.y, b.v.y));
+  }
+};
+// A 16-byte packet as pairs.
+template <typename T>
+union PairPacket {
+  static constexpr int N = 16 / sizeof(Pair<T>);
+  uint4 u;
+  Pair<T> p[N];
+  __device__ __forceinline__ PairPacket() {}
+};
+
+__device__ __forceinline__ float warp_redux_max(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// (maximum, sum exp((x - max) / T), sum exp(x - max)) of a set of logits.
+struct Stat {
+  float m, z, z1;
+};
+// Joins the sets of the lanes; WIDTH of them differ (lane l holds set l % WIDTH).
+template <typename T, bool TWO, int WIDTH>
+__device__ __forceinline__ Stat join(Stat s, float inv_t) {
+  Stat r;
+  r.m = warp_redux_max(s.m);
+  const float d = s.m == -INFINITY ? 0.f : s.m - r.m;  // an empty set's sum is 0, or NaN
+  r.z = s.z * exp_of<T>(d * inv_t);
+  r.z1 = TWO ? s.z1 * exp_of<T>(d) : 0.f;
+#pragma unroll
+  for (int o = WIDTH / 2; o > 0; o >>= 1) {
+    r.z += __shfl_xor_sync(0xffffffffu, r.z, o);
+    if (TWO) r.z1 += __shfl_xor_sync(0xffffffffu, r.z1, o);
+  }
+  return r;
+}
+
+template <typename T, bool TWO, int THREADS, int KP, int MIN_CTAS>
+__global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
+    const T* logits, int64_t lstride, T* grad, int64_t gstride, int stage_bytes, int log_c,
+    RowArgs a) {
+  using PK = PairPacket<T>;
+  constexpr int VN = 16 / (int)sizeof(T);
+  constexpr int NP = PK::N;
+  constexpr bool kKeep = !(TWO && sizeof(T) == 2);
+  constexpr int kWarps = THREADS / 32;
+  extern __shared__ __align__(128) unsigned char ring[];
+  float* picked = reinterpret_cast<float*>(ring + kStages * stage_bytes);  // [list]
+  __shared__ __align__(8) uint64_t full[kStages];
+  __shared__ __align__(8) uint64_t xbar[2];
+  __shared__ __align__(16) float4 xch[2][8];
+  __shared__ Stat wred[kWarps];
+  __shared__ float wloss[kWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int C = 1 << log_c, rank = (int)ptx::cluster_ctarank();
+  const int64_t first = blockIdx.x >> log_c, step = gridDim.x >> log_c;
+  const bool loader = tid == THREADS - 32;  // the last warp's first lane starts the loads
+
+  // A row's 16-byte packets and this CTA's share of them.
+  struct Slice {
+    int head, packets, start, count;
+  };
+  auto slice_of = [&](const T* src) {
+    Slice s;
+    s.head = (int)((0u - (unsigned)reinterpret_cast<uintptr_t>(src)) & 15u) / (int)sizeof(T);
+    if (s.head > a.n_cols) s.head = a.n_cols;
+    s.packets = (int)((unsigned)(a.n_cols - s.head) / (unsigned)VN);
+    const int per = (s.packets + C - 1) >> log_c;
+    s.start = rank * per;
+    const int left = s.packets - s.start;
+    s.count = left < per ? (left < 0 ? 0 : left) : per;
+    return s;
+  };
+  auto issue = [&](int64_t row, int q) {  // loader: this CTA's slice of a row into stage q
+    if (row >= a.n_rows) return;
+    const T* src = logits + row * lstride;
+    const Slice s = slice_of(src);
+    ptx::fence_proxy_async_smem();
+    if (s.count > 0) {
+      ptx::mbar_arrive_expect_tx(&full[q], (uint32_t)s.count * 16u);
+      ptx::bulk_g2s(ring + q * stage_bytes, src + s.head + s.start * VN, (uint32_t)s.count * 16u,
+                    &full[q]);
+    } else {
+      ptx::mbar_arrive(&full[q]);
+    }
+  };
+  if (tid == 0) {
+    for (int q = 0; q < kStages; ++q) ptx::mbar_init(&full[q], 1);
+    ptx::mbar_init(&xbar[0], 1);
+    ptx::mbar_init(&xbar[1], 1);
+    ptx::fence_mbar_init();
+  }
+  if (C > 1) ptx::cluster_sync();
+  else __syncthreads();
+  if (loader)
+    for (int q = 0; q < kStages; ++q) issue(first + q * step, q);
+
+  const float inv_n = 1.0f / count_valid(a);
+  const float inv_t = a.inv_t;
+  const float ct_row = inv_t * kLog2e;  // exponent of 2 per unit of logit
+  bool ok = true;
+  double total = 0.0;
+  int q = 0, phase = 0, xb = 0, xphase = 0;
+  // What the row brings besides its logits is read one row ahead.
+  int state = 0, my_id = -1;
+  float my_p = 0.f;
+  auto read_ahead = [&](int64_t row) {
+    if (row >= a.n_rows) return;
+    state = a.state[row];
+    if (tid < a.list) {
+      my_id = a.ids[row * a.list + tid];
+      my_p = a.probs[row * a.list + tid];
+    }
+  };
+  read_ahead(first);
+  for (int64_t row = first; row < a.n_rows; row += step) {
+    const T* src = logits + row * lstride;
+    const Slice sl = slice_of(src);
+    const int row_state = state, id = my_id;
+    const float p_id = my_p;
+    float xs = -INFINITY;  // an element outside the packets
+    int xs_at = -1;
+    if (rank == 0 && warp < 2) {
+      const int tail = sl.head + sl.packets * VN;
+      if (tid < sl.head) xs_at = tid;
+      else if (tid >= 32 && tid - 32 < a.n_cols - tail) xs_at = tail + tid - 32;
+      if (xs_at >= 0) xs = Elt<T>::to_f(src[xs_at]);
+    }
+    ok = ptx::mbar_wait(&full[q], (uint32_t)phase, ok ? (1u << 26) : 1u) && ok;
+    const unsigned char* stage = ring + q * stage_bytes;
+    PK p[KP];
+#pragma unroll
+    for (int u = 0; u < KP; ++u) {
+      const int v = tid + u * THREADS;
+      constexpr uint32_t w = Pair<T>::kNegInf;
+      p[u].u = make_uint4(w, w, w, w);
+      if (v < sl.count) p[u].u = *reinterpret_cast<const uint4*>(stage + v * 16);
+    }
+    // Listed elements of this slice: the same thread handles a listed place all through.
+    auto mine = [&](int c) {  // whether element c is this CTA's
+      const unsigned off = (unsigned)(c - sl.head);
+      if (c < 0) return false;
+      if (off >= (unsigned)(sl.packets * VN)) return rank == 0;
+      return off / VN - (unsigned)sl.start < (unsigned)sl.count;
+    };
+    auto value = [&](int c) {  // its logit
+      const unsigned off = (unsigned)(c - sl.head);
+      if (off >= (unsigned)(sl.packets * VN)) return Elt<T>::to_f(src[c]);
+      return Elt<T>::to_f(reinterpret_cast<const T*>(stage)[(int)off - sl.start * VN]);
+    };
+    const bool has = mine(id);
+    const float x_id = has ? value(id) : 0.f;
+    for (int j = tid + THREADS; j < a.list; j += THREADS) {
+      const int c = a.ids[row * a.list + j];
+      if (mine(c)) picked[j] = value(c);
+    }
+    // This thread's maximum and exponentials.
+    float my_m;
+    {
+      Pair<T> top = p[0].p[0];
+#pragma unroll
+      for (int k = 1; k < KP * NP; ++k) top.take_max(p[k / NP].p[k % NP]);
+      const float2 f = top.f();
+      my_m = fmaxf(fmaxf(f.x, f.y), xs);
+    }
+    const float base = my_m == -INFINITY ? 0.f : my_m;
+    const float2 nb_t = make_float2(-base * ct_row, -base * ct_row);
+    const float2 nb_1 = make_float2(-base * kLog2e, -base * kLog2e);
+    auto exp_pair = [&](float2 x, float2& f, float2& f1) {
+      if constexpr (sizeof(T) == 2) {
+        const float2 t = __ffma2_rn(x, make_float2(ct_row, ct_row), nb_t);
+        f = make_float2(ex2f(t.x), ex2f(t.y));
+        if constexpr (TWO) {
+          const float2 t1 = __ffma2_rn(x, make_float2(kLog2e, kLog2e), nb_1);
+          f1 = make_float2(ex2f(t1.x), ex2f(t1.y));
+        }
+      } else {
+        const float2 d = __fadd2_rn(x, make_float2(-base, -base));
+        f = exp2_of(TWO ? __fmul2_rn(d, make_float2(inv_t, inv_t)) : d);
+        if constexpr (TWO) f1 = exp2_of(d);
+      }
+    };
+    float2 e[KP][kKeep ? NP : 1], e1[KP][kKeep && TWO ? NP : 1];
+    float2 es, es1 = make_float2(0.f, 0.f), z = make_float2(0.f, 0.f), z1 = z;
+    exp_pair(make_float2(xs, -INFINITY), es, es1);
+    z.x = es.x;
+    z1.x = es1.x;
+#pragma unroll
+    for (int u = 0; u < KP; ++u)
+#pragma unroll
+      for (int k = 0; k < NP; ++k) {
+        float2 f, f1;
+        exp_pair(p[u].p[k].f(), f, f1);
+        z = __fadd2_rn(z, f);
+        if constexpr (TWO) z1 = __fadd2_rn(z1, f1);
+        if constexpr (kKeep) {
+          e[u][k] = f;
+          if constexpr (TWO) e1[u][k] = f1;
+        }
+      }
+    Stat st = join<T, TWO, 32>(Stat{my_m, z.x + z.y, TWO ? z1.x + z1.y : 0.f}, inv_t);
+    if (lane == 0) wred[warp] = st;
+    __syncthreads();  // the stage has been read by all
+    if (loader) issue(row + kStages * step, q);
+    if (C == 1 || warp == 0) st = join<T, TWO, kWarps>(wred[lane & (kWarps - 1)], inv_t);
+    if (C > 1) {
+      if (warp == 0) {
+        if (lane == 0) ptx::mbar_arrive_expect_tx(&xbar[xb], (uint32_t)C * 16u);
+        if (lane < C)
+          ptx::st_async16(ptx::peer_smem(&xch[xb][rank], (uint32_t)lane),
+                          make_float4(st.m, st.z, st.z1, 0.f),
+                          ptx::peer_smem(&xbar[xb], (uint32_t)lane));
+        __syncwarp();
+      }
+      read_ahead(row + step);
+      ok = ptx::mbar_wait(&xbar[xb], (uint32_t)xphase, ok ? (1u << 26) : 1u) && ok;
+      const float4 f = xch[xb][lane & (C - 1)];
+      const bool copy = (lane & 7) >= C;  // of a smaller cluster: counted once
+      st = join<T, TWO, 8>(Stat{f.x, copy ? 0.f : f.y, copy ? 0.f : f.z}, inv_t);
+    } else {
+      read_ahead(row + step);
+    }
+    if (!ok) st.z = st.z1 = __int_as_float(0x7fc00000);  // a wait ran out: the row is poisoned
+    const float hw = (row_state & kHard) ? a.hard_weight : 0.f;
+    const float sw = (row_state & kSoft) ? 1.f - a.hard_weight : 0.f;
+    const float ct = sw * a.temperature * a.loss_scale * inv_n, c1 = hw * a.loss_scale * inv_n;
+    const float kt = TWO ? ct / st.z : (ct + c1) / st.z, k1 = TWO ? c1 / st.z1 : 0.f;
+    const bool plain = row_state == kSkip || row_state == kBad;
+    const float fill = row_state == kBad || !ok ? __int_as_float(0x7fc00000) : 0.f;
+
+    T* dst = grad + row * gstride;
+    T* out = dst + sl.head + sl.start * VN;
+    if (grad) {
+      if (plain) {
+        PK o;
+#pragma unroll
+        for (int k = 0; k < NP; ++k) o.p[k].set(make_float2(fill, fill));
+#pragma unroll
+        for (int u = 0; u < KP; ++u) {
+          const int v = tid + u * THREADS;
+          if (v < sl.count) __stcs(reinterpret_cast<uint4*>(out) + v, o.u);
+        }
+        if (xs_at >= 0) dst[xs_at] = Elt<T>::from_f(fill);
+      } else {
+        const bool none = my_m == -INFINITY;
+        // Without kept exponentials only the single element's were formed against base.
+        // (A thread with nothing but -inf: 0, or NaN where the row's sum is.)
+        const float ft = (none ? 0.f : exp_of<T>((base - st.m) * inv_t)) * kt;
+        const float f1 = (none || !TWO ? 0.f : exp_of<T>(base - st.m)) * k1;
+        const float wt = kKeep ? ft : kt, w1 = kKeep ? f1 : k1;
+        const float2 ot = make_float2(-st.m * ct_row, -st.m * ct_row);
+        const float2 o1 = make_float2(-st.m * kLog2e, -st.m * kLog2e);
+#pragma unroll
+        for (int u = 0; u < KP; ++u) {
+          const int v = tid + u * THREADS;
+          PK o;
+#pragma unroll
+          for (int k = 0; k < NP; ++k) {
+            float2 f, g1 = make_float2(0.f, 0.f);
+            if constexpr (kKeep) {
+              f = e[u][k];
+              if constexpr (TWO) g1 = e1[u][k];
+            } else {
+              const float2 x = p[u].p[k].f();
+              const float2 t = __ffma2_rn(x, make_float2(ct_row, ct_row), ot);
+              const float2 t1 = __ffma2_rn(x, make_float2(kLog2e, kLog2e), o1);
+              f = make_float2(ex2f(t.x), ex2f(t.y));
+              g1 = make_float2(ex2f(t1.x), ex2f(t1.y));
+            }
+            float2 g = __fmul2_rn(f, make_float2(wt, wt));
+            if constexpr (TWO) g = __ffma2_rn(g1, make_float2(w1, w1), g);
+            o.p[k].set(g);
+          }
+          if (v < sl.count) __stcs(reinterpret_cast<uint4*>(out) + v, o.u);
+        }
+        if (xs_at >= 0) dst[xs_at] = Elt<T>::from_f(TWO ? fmaf(es.x, ft, es1.x * f1) : es.x * ft);
+      }
+    }
+    // The row's loss, the part of this CTA's listed elements.
+    float l = 0.f;
+    auto listed_loss = [&](int j, float x, float pj) {
+      const float d = x - st.m;
+      if (sw > 0.f && pj != 0.f) l -= sw * a.temperature * pj * d;
+      if (hw > 0.f && j == a.list - 1) l -= hw * d;
+    };
+    if (!plain) {
+      if (has) listed_loss(tid, x_id, p_id);
+      for (int j = tid + THREADS; j < a.list; j += THREADS)
+        if (mine(a.ids[row * a.list + j])) listed_loss(j, picked[j], a.probs[row * a.list + j]);
+    }
+    if (warp * 32 < a.list) {
+      l = warp_sum(l);
+      if (lane == 0) wloss[warp] = l;
+    }
+    __syncthreads();  // the listed places are written over the dense values
+    auto listed_grad = [&](int j, int c, float x, float pj) {
+      const float d = x - st.m;
+      float g = kt * exp_of<T>(d * inv_t) - ct * pj;
+      if constexpr (TWO) g = fmaf(k1, exp_of<T>(d), g);
+      if ((row_state & kHard) && j == a.list - 1) g -= c1;
+      dst[c] = Elt<T>::from_f(g);
+    };
+    if (grad && !plain) {
+      if (has) listed_grad(tid, id, x_id, p_id);
+      for (int j = tid + THREADS; j < a.list; j += THREADS) {
+        const int c = a.ids[row * a.list + j];
+        if (mine(c)) listed_grad(j, c, picked[j], a.probs[row * a.list + j]);
+      }
+    }
+    if (tid == 0) {
+      float s = 0.f;
+      for (int w = 0; w < kWarps && w * 32 < a.list; ++w) s += wloss[w];
+      if (plain) s = fill;
+      else if (rank == 0) {  // a part of weight 0 is left out, even where it is infinite
+        if (sw > 0.f) s += sw * a.temperature * a.temperature * (a.entropy[row] + logf(st.z));
+        if (hw > 0.f) s += hw * logf(TWO ? st.z1 : st.z);
+      }
+      total += (double)s;
+    }
+    if (++q == kStages) {
+      q = 0;
+      phase ^= 1;
+    }
+    xphase ^= xb;
+    xb ^= 1;
+  }
+  if (C > 1) ptx::cluster_sync();  // nobody's shared memory is written after its CTA is gone
+  finish_loss(a, 1.0f / inv_n, total);
+}
+
+template <typename T, bool TWO, int THREADS, int KP, int MIN_CTAS>
+int launch_rows(const T* lp, int64_t ls, T* gp, int64_t gs, int log_c, int stage_bytes,
+                const RowArgs& a, cudaStream_t st) {
+  auto kern = distill_rows<T, TWO, THREADS, KP, MIN_CTAS>;
+  const int smem = kStages * stage_bytes + (a.list + 3) / 4 * 16;
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const int cluster = 1 << log_c;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)cluster);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  // The grid is what the GPU holds at once (clusters of 8 do not fill every SM).
+  int most = 0;
+  if (cudaOccupancyMaxActiveClusters(&most, kern, &cfg) != cudaSuccess || most < 1) {
+    cudaGetLastError();
+    most = 1;
+  }
+  if (most * cluster > num_sms() * kMaxRowCtasPerSm) most = num_sms() * kMaxRowCtasPerSm / cluster;
+  const int64_t clusters = a.n_rows < most ? a.n_rows : most;
+  cfg.gridDim = dim3((unsigned)((clusters < 1 ? 1 : clusters) * cluster));
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, lp, ls, gp, gs, stage_bytes, log_c, a);
+  if (e != cudaSuccess) return fail(FK_ERR_LAUNCH, "fk_distill(rows): %s", cudaGetErrorString(e));
+  return launch_status("fk_distill(rows)");
+}
+
+template <typename T, bool TWO>
+int rows_two(const T* lp, int64_t ls, T* gp, int64_t gs, const RowArgs& a, cudaStream_t st) {
+  // Cluster: as many CTAs as a row needs for slices of at most 32 KB, more (down to 4 KB)
+  // while the rows are too few for the SMs.
+  const int64_t packets = (int64_t)a.n_cols * sizeof(T) / 16 + 1;
+  int lc = 0;
+  while (lc < 3 && packets > (int64_t)2048 << lc) ++lc;
+  while (lc < 3 && (a.n_rows << lc) < num_sms() && (packets >> lc) > 512) ++lc;
+  const int64_t per = (packets + ((int64_t)1 << lc) - 1) >> lc;
+  const int bytes = (int)(per < 1 ? 16 : per * 16);
+  if (per <= 128) return launch_rows<T, TWO, 128, 1, 8>(lp, ls, gp, gs, lc, bytes, a, st);
+  if (per <= 512) return launch_rows<T, TWO, 128, 4, 8>(lp, ls, gp, gs, lc, bytes, a, st);
+  if (per <= 1024) return launch_rows<T, TWO, 256, 4, 4>(lp, ls, gp, gs, lc, bytes, a, st);
+  if (per <= 2048) return launch_rows<T, TWO, 512, 4, 2>(lp, ls, gp, gs, lc, bytes, a, st);
+  return launch_rows<T, TWO, 512, 8, 1>(lp, ls, gp, gs, lc, bytes, a, st);
 }
 
 template <typename T>
 int rows_t(const void* logits, int64_t ls, void* grad, int64_t gs, const RowArgs& a,
            cudaStream_t st) {
-  const int64_t most = (int64_t)num_sms() * kRowCtasPerSm;
+  const T* lp = static_cast<const T*>(logits);
+  T* gp = static_cast<T*>(grad);
+  const int64_t apart = reinterpret_cast<intptr_t>(lp) - reinterpret_cast<intptr_t>(gp);
+  const bool same_offset = !gp || (apart % 16 == 0 && (ls - gs) * (int64_t)sizeof(T) % 16 == 0);
+  const int64_t packets = (int64_t)a.n_cols * sizeof(T) / 16 + 1;
+  if (same_offset && packets <= 8 * 4096) {
+    if (a.temperature == 1.0f) return rows_two<T, false>(lp, ls, gp, gs, a, st);
+    return rows_two<T, true>(lp, ls, gp, gs, a, st);
+  }
+  const int64_t most = (int64_t)num_sms() * 8;
   const int grid = (int)(a.n_rows < most ? a.n_rows : most);
-  distill_rows_generic<T><<<grid < 1 ? 1 : grid, kRowThreads, 0, st>>>(
-      static_cast<const T*>(logits), ls, static_cast<T*>(grad), gs, a);
+  distill_rows_generic<T><<<grid < 1 ? 1 : grid, kGenericThreads, 0, st>>>(lp, ls, gp, gs, a);
   return launch_status("fk_distill(rows)");
 }
 
@@ -391,7 +854,7 @@ extern "C" int fk_distill(const void* logits, int64_t row_stride, void* grad,
   a.state = ws.state;
   a.ids = ws.ids;
   a.probs = ws.probs;
-  a.loss_rows = ws.loss_rows;
+  a.sums = ws.sums;
   a.ticket = ws.ticket;
   a.loss = loss;
   a.err = err_flag;

@@ -101,5 +101,29 @@ __device__ __forceinline__ float ld_dsmem_f32(uint32_t cluster_addr) {
   return v;
 }
 
+// Address of the same shared object in CTA `rank`, from a generic pointer to this CTA's.
+__device__ __forceinline__ uint32_t peer_smem(const void* p, uint32_t rank) {
+  return mapa(smem_u32(p), rank);
+}
+// 16 bytes into a CTA of this cluster; completes 16 bytes on an mbarrier of that CTA.
+__device__ __forceinline__ void st_async16(uint32_t cluster_addr, float4 v, uint32_t cluster_bar) {
+  asm volatile(
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::
+          "r"(cluster_addr),
+      "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(cluster_bar)
+      : "memory");
+}
+
+// ---------------------------------------------------------------- dependent launches
+// In a kernel launched with programmatic stream serialization: waits until the kernel before
+// it in the stream is done and its writes are visible (returns at once in any other launch).
+__device__ __forceinline__ void wait_for_previous_kernel() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// Lets the next kernel in the stream start once every CTA has come here or has ended.
+__device__ __forceinline__ void let_next_kernel_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 }  // namespace ptx
 }  // namespace fk
