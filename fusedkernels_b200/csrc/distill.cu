@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kMaxSlots = 1024;
 constexpr int kTeacherWarps = 8;
-constexpr int kTeacherCtas = 64;   // partial counts that every CTA of the second kernel adds up
+constexpr int kTeacherCtas = 512;  // partial counts that every CTA of the second kernel adds up
 constexpr int kMaxRowCtasPerSm = 16;
 // Row states.
 constexpr int kSkip = 0, kSoft = 1, kHard = 2, kBad = 4;
@@ -216,11 +216,25 @@ __device__ __forceinline__ float count_valid(const RowArgs& a) {
   return (float)(n < 1 ? 1 : n);
 }
 
-// Thread 0 leaves the loss of its CTA's rows; the CTA that ends last adds them up in a fixed
-// order (at most 16 per SM).
+// Sum over the CTA's threads in a fixed order (valid in thread 0).
+__device__ __forceinline__ double block_total(double s) {
+  __shared__ double red[32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  s = 0.0;
+  if (threadIdx.x == 0)
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) s += red[i];
+  return s;
+}
+
+// Every thread brings its part of the loss of the CTA's rows; the CTA that ends last adds the
+// CTAs' sums up in a fixed order (at most 16 per SM).
 __device__ __forceinline__ void finish_loss(const RowArgs& a, float n, double mine) {
   __shared__ bool last;
-  __shared__ double red[32];
+  mine = block_total(mine);
   if (threadIdx.x == 0) {
     a.sums[blockIdx.x] = mine;
     __threadfence();
@@ -231,16 +245,12 @@ __device__ __forceinline__ void finish_loss(const RowArgs& a, float n, double mi
   __threadfence();
   double s = 0.0;
   for (int i = threadIdx.x; i < (int)gridDim.x; i += blockDim.x) s += __ldcg(a.sums + i);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-  __syncthreads();
+  s = block_total(s);
+  int bad = 0;
+  for (int i = threadIdx.x; i < a.teacher_ctas; i += blockDim.x) bad |= a.valid[i].y;
+  bad = __syncthreads_or(bad);
   if (threadIdx.x == 0) {
-    s = 0.0;
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) s += red[i];
     *a.loss = (float)(s / (double)n);
-    int bad = 0;
-    for (int i = 0; i < a.teacher_ctas; ++i) bad |= a.valid[i].y;
     *a.err = bad != 0;
   }
 }
@@ -263,7 +273,7 @@ __global__ void __launch_bounds__(kGenericThreads) distill_rows_generic(
     const int state = a.state[row];
     if (state == kSkip || state == kBad) {
       const float z = state == kBad ? __int_as_float(0x7fc00000) : 0.f;
-      total += (double)z;
+      if (threadIdx.x == 0) total += (double)z;
       if (dst)
         for (int c = threadIdx.x; c < a.n_cols; c += blockDim.x) dst[c] = Elt<T>::from_f(z);
       continue;
@@ -444,7 +454,6 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
   __shared__ __align__(8) uint64_t xbar[2];
   __shared__ __align__(16) float4 xch[2][8];
   __shared__ Stat wred[kWarps];
-  __shared__ float wloss[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = 1 << log_c, rank = (int)ptx::cluster_ctarank();
   const int64_t first = blockIdx.x >> log_c, step = gridDim.x >> log_c;
@@ -497,11 +506,12 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
   int q = 0, phase = 0, xb = 0, xphase = 0;
   // What the row brings besides its logits is read one row ahead.
   int state = 0, my_id = -1;
-  float my_p = 0.f;
+  float my_p = 0.f, entropy = 0.f;
   auto read_ahead = [&](int64_t row) {
     if (row >= a.n_rows) return;
     state = a.state[row];
-    if (tid < a.list) {
+    if (tid == THREADS - 1) entropy = a.entropy[row];
+    if (warp * 32 < a.list && tid < a.list) {
       my_id = a.ids[row * a.list + tid];
       my_p = a.probs[row * a.list + tid];
     }
@@ -511,7 +521,7 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
     const T* src = logits + row * lstride;
     const Slice sl = slice_of(src);
     const int row_state = state, id = my_id;
-    const float p_id = my_p;
+    const float p_id = my_p, row_entropy = entropy;
     float xs = -INFINITY;  // an element outside the packets
     int xs_at = -1;
     if (rank == 0 && warp < 2) {
@@ -618,7 +628,7 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
     const float hw = (row_state & kHard) ? a.hard_weight : 0.f;
     const float sw = (row_state & kSoft) ? 1.f - a.hard_weight : 0.f;
     const float ct = sw * a.temperature * a.loss_scale * inv_n, c1 = hw * a.loss_scale * inv_n;
-    const float kt = TWO ? ct / st.z : (ct + c1) / st.z, k1 = TWO ? c1 / st.z1 : 0.f;
+    const float kt = __fdividef(TWO ? ct : ct + c1, st.z), k1 = TWO ? __fdividef(c1, st.z1) : 0.f;
     const bool plain = row_state == kSkip || row_state == kBad;
     const float fill = row_state == kBad || !ok ? __int_as_float(0x7fc00000) : 0.f;
 
@@ -670,47 +680,37 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
         if (xs_at >= 0) dst[xs_at] = Elt<T>::from_f(TWO ? fmaf(es.x, ft, es1.x * f1) : es.x * ft);
       }
     }
-    // The row's loss, the part of this CTA's listed elements.
-    float l = 0.f;
-    auto listed_loss = [&](int j, float x, float pj) {
-      const float d = x - st.m;
-      if (sw > 0.f && pj != 0.f) l -= sw * a.temperature * pj * d;
-      if (hw > 0.f && j == a.list - 1) l -= hw * d;
-    };
-    if (!plain) {
-      if (has) listed_loss(tid, x_id, p_id);
-      for (int j = tid + THREADS; j < a.list; j += THREADS)
-        if (mine(a.ids[row * a.list + j])) listed_loss(j, picked[j], a.probs[row * a.list + j]);
-    }
-    if (warp * 32 < a.list) {
-      l = warp_sum(l);
-      if (lane == 0) wloss[warp] = l;
-    }
     __syncthreads();  // the listed places are written over the dense values
-    auto listed_grad = [&](int j, int c, float x, float pj) {
+    // The listed elements of this CTA: their part of the loss, and their gradient.  A part of
+    // the loss whose weight is 0 is left out, even where it is infinite.
+    float l = 0.f;
+    auto listed = [&](int j, int c, float x, float pj) {
       const float d = x - st.m;
-      float g = kt * exp_of<T>(d * inv_t) - ct * pj;
-      if constexpr (TWO) g = fmaf(k1, exp_of<T>(d), g);
-      if ((row_state & kHard) && j == a.list - 1) g -= c1;
-      dst[c] = Elt<T>::from_f(g);
+      const bool label = j == a.list - 1;
+      if (sw > 0.f && pj != 0.f) l -= sw * a.temperature * pj * d;
+      if (hw > 0.f && label) l -= hw * d;
+      if (grad) {
+        float g = kt * exp_of<T>(d * inv_t) - ct * pj;
+        if constexpr (TWO) g = fmaf(k1, exp_of<T>(d), g);
+        if (label) g -= c1;
+        dst[c] = Elt<T>::from_f(g);
+      }
     };
-    if (grad && !plain) {
-      if (has) listed_grad(tid, id, x_id, p_id);
+    if (!plain && warp * 32 < a.list) {
+      if (has) listed(tid, id, x_id, p_id);
       for (int j = tid + THREADS; j < a.list; j += THREADS) {
         const int c = a.ids[row * a.list + j];
-        if (mine(c)) listed_grad(j, c, picked[j], a.probs[row * a.list + j]);
+        if (mine(c)) listed(j, c, picked[j], a.probs[row * a.list + j]);
       }
     }
-    if (tid == 0) {
-      float s = 0.f;
-      for (int w = 0; w < kWarps && w * 32 < a.list; ++w) s += wloss[w];
-      if (plain) s = fill;
-      else if (rank == 0) {  // a part of weight 0 is left out, even where it is infinite
-        if (sw > 0.f) s += sw * a.temperature * a.temperature * (a.entropy[row] + logf(st.z));
-        if (hw > 0.f) s += hw * logf(TWO ? st.z1 : st.z);
+    if (rank == 0 && tid == THREADS - 1) {
+      if (plain) l = fill;
+      else {
+        if (sw > 0.f) l += sw * a.temperature * a.temperature * (row_entropy + logf(st.z));
+        if (hw > 0.f) l += hw * logf(TWO ? st.z1 : st.z);
       }
-      total += (double)s;
     }
+    total += (double)l;
     if (++q == kStages) {
       q = 0;
       phase ^= 1;
@@ -766,8 +766,8 @@ int rows_two(const T* lp, int64_t ls, T* gp, int64_t gs, const RowArgs& a, cudaS
   const int bytes = (int)(per < 1 ? 16 : per * 16);
   if (per <= 128) return launch_rows<T, TWO, 128, 1, 8>(lp, ls, gp, gs, lc, bytes, a, st);
   if (per <= 512) return launch_rows<T, TWO, 128, 4, 8>(lp, ls, gp, gs, lc, bytes, a, st);
-  if (per <= 1024) return launch_rows<T, TWO, 256, 4, 4>(lp, ls, gp, gs, lc, bytes, a, st);
-  if (per <= 2048) return launch_rows<T, TWO, 512, 4, 2>(lp, ls, gp, gs, lc, bytes, a, st);
+  if (per <= 1024) return launch_rows<T, TWO, 128, 8, 4>(lp, ls, gp, gs, lc, bytes, a, st);
+  if (per <= 2048) return launch_rows<T, TWO, 256, 8, 2>(lp, ls, gp, gs, lc, bytes, a, st);
   return launch_rows<T, TWO, 512, 8, 1>(lp, ls, gp, gs, lc, bytes, a, st);
 }
 
