@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kMaxSlots = 1024;
 constexpr int kTeacherWarps = 8;
-constexpr int kTeacherCtas = 512;  // partial counts that every CTA of the second kernel adds up
+constexpr int kTeacherCtas = 1024;  // partial counts that every CTA of the second kernel adds up
 constexpr int kMaxRowCtasPerSm = 16;
 // Row states.
 constexpr int kSkip = 0, kSoft = 1, kHard = 2, kBad = 4;
@@ -67,6 +67,7 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) distill_teacher(
   int* ids = smem + warp * (2 * k + table);
   float* p = reinterpret_cast<float*>(ids + k);
   int* hash = ids + 2 * k;
+  ptx::let_next_kernel_start();
   if (threadIdx.x == 0) {
     valid_rows = bad_rows = 0;
     if (blockIdx.x == 0) *ws.ticket = 0;
@@ -78,21 +79,27 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) distill_teacher(
     const int64_t y = targets ? targets[row] : -1;
     const bool ignored = targets && y == ignore_index;
     bool bad = targets && !ignored && (y < 0 || y >= n_cols);
-    for (int i = lane; i < table; i += 32) hash[i] = -1;
-    __syncwarp();
     float m = -INFINITY;
     bool twice = false, nan = false;
+#pragma unroll 4
     for (int j = lane; j < k; j += 32) {
       const int64_t id = idx[row * k + j];
+      const float v = Elt<T>::to_f(top[row * k + j]);
       const bool out = id >= n_cols;
       bad = bad || (out && !ignored);
       const int c = (id < 0 || out) ? -1 : (int)id;
-      const float v = Elt<T>::to_f(top[row * k + j]);
       ids[j] = c;
       p[j] = v;
       if (c >= 0) {
         m = fmaxf(m, v);
         nan = nan || v != v;
+      }
+    }
+    for (int i = lane; i < table; i += 32) hash[i] = -1;
+    __syncwarp();
+    for (int j = lane; j < k; j += 32) {
+      const int c = ids[j];
+      if (c >= 0) {
         unsigned at = ((unsigned)c * 2654435761u) & (unsigned)(table - 1);
         for (;;) {  // at most k ids in a table of at least 2k places: a free one is found
           const int old = atomicCAS(&hash[at], -1, c);
@@ -332,20 +339,21 @@ __global__ void __launch_bounds__(kGenericThreads) distill_rows_generic(
 
 // ------------------------------------------------------------------ rows, 16-byte packets
 // A cluster of 1, 2, 4 or 8 CTAs takes a row; each CTA has a slice of its 16-byte packets, at
-// most KP per thread.  Slices arrive through a ring of kStages shared-memory buffers filled by
-// cp.async.bulk, so the next rows are on their way while a row is worked on; a slice then lies
-// in registers, and its buffer is refilled as soon as every thread has taken its packets.
+// most KP per thread.  A slice arrives in a shared-memory buffer by cp.async.bulk, moves to
+// registers, and its buffer is refilled with the next row's as soon as every thread has taken
+// its packets: the next row is on its way while this one is worked on.
 //
-// Each logit is exponentiated once: e = exp((x - m_t) / T) with the thread's own maximum m_t
-// stays in registers, and after the row's maximum m and sum z are known the gradient is
-// e * [exp((m_t - m) / T) * k / z].  (With two temperatures and 16-bit logits the registers do
-// not hold both exponentials, and they are formed again from the logits.)  The CTAs of a row
-// exchange (m, z) by st.async into each other's shared memory.
+// A thread forms the sum of exp((x - m_t) / T) with its own maximum m_t; the CTAs of a row
+// exchange (m, z) by st.async into each other's shared memory.  16-bit packets stay in
+// registers and the gradient's exponentials are formed anew: keeping the first ones in 32 bits
+// takes twice the registers, half as many rows are then in flight, and their latency shows
+// (810 against 717 us at 8192 x 128256 bf16).  32-bit packets give their registers to their
+// exponentials, which the gradient only scales.
 //
 // Elements before the first and after the last 16-byte boundary of a row (any odd width or
 // offset) are taken singly by the first CTA.  Logits and gradient have to have the same
 // offset from a 16-byte boundary in every row; other layouts take the generic kernel.
-constexpr int kStages = 3;
+constexpr int kMaxStages = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2f(float x) {
@@ -360,7 +368,7 @@ __device__ __forceinline__ float exp_of(float d) { return ex2f(d * kLog2e); }
 template <>
 __device__ __forceinline__ float exp_of<float>(float d) { return expf(d); }
 
-// exp of a pair.  16 bits: as above.  32 bits: 2^(d log2 e) with the product in two parts,
+// exp in 32 bits: 2^(d log2 e) with the product in two parts,
 // hi + lo (log2 e = kLog2e + kLog2eLow, the roundings of the products caught by FMAs), so that
 // the error stays that of ex2 (2 ulp) for any d: 2^hi * (1 + lo ln 2), lo being below 2^-16.
 // d is held at -200 from below (2^hi is 0 there), so that -inf does not meet its own residual.
@@ -371,13 +379,12 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float2 exp2_of(float2 d) {
-  d = make_float2(max_or_nan(d.x, -200.f), max_or_nan(d.y, -200.f));
-  const float2 hi = __fmul2_rn(d, make_float2(kLog2e, kLog2e));
-  float2 lo = __ffma2_rn(d, make_float2(kLog2e, kLog2e), make_float2(-hi.x, -hi.y));
-  lo = __ffma2_rn(d, make_float2(kLog2eLow, kLog2eLow), lo);
-  const float2 p = make_float2(ex2f(hi.x), ex2f(hi.y));
-  return __ffma2_rn(__fmul2_rn(p, make_float2(kLn2, kLn2)), lo, p);
+__device__ __forceinline__ float exp2_of(float d) {
+  d = max_or_nan(d, -200.f);
+  const float hi = d * kLog2e;
+  const float lo = fmaf(d, kLog2eLow, fmaf(d, kLog2e, -hi));
+  const float p = ex2f(hi);
+  return fmaf(p * kLn2, lo, p);
 }
 
 template <typename T> struct Pair;  // two neighbouring elements
@@ -419,44 +426,48 @@ __device__ __forceinline__ float warp_redux_max(float v) {
   return r;
 }
 
+// What a row needs: softmax at one temperature, at two (the soft part's and 1), or at 2 and 1,
+// where exp(d) is the square of exp(d / 2).
+enum Mode { kOne, kTwo, kSquare };
+
 // (maximum, sum exp((x - max) / T), sum exp(x - max)) of a set of logits.
 struct Stat {
   float m, z, z1;
 };
 // Joins the sets of the lanes; WIDTH of them differ (lane l holds set l % WIDTH).
-template <typename T, bool TWO, int WIDTH>
+template <typename T, Mode M, int WIDTH>
 __device__ __forceinline__ Stat join(Stat s, float inv_t) {
   Stat r;
   r.m = warp_redux_max(s.m);
   const float d = s.m == -INFINITY ? 0.f : s.m - r.m;  // an empty set's sum is 0, or NaN
   r.z = s.z * exp_of<T>(d * inv_t);
-  r.z1 = TWO ? s.z1 * exp_of<T>(d) : 0.f;
+  r.z1 = M != kOne ? s.z1 * exp_of<T>(d) : 0.f;
 #pragma unroll
   for (int o = WIDTH / 2; o > 0; o >>= 1) {
     r.z += __shfl_xor_sync(0xffffffffu, r.z, o);
-    if (TWO) r.z1 += __shfl_xor_sync(0xffffffffu, r.z1, o);
+    if (M != kOne) r.z1 += __shfl_xor_sync(0xffffffffu, r.z1, o);
   }
   return r;
 }
 
-template <typename T, bool TWO, int THREADS, int KP, int MIN_CTAS>
+template <typename T, Mode M, bool KEEP, int THREADS, int KP, int MIN_CTAS>
 __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
-    const T* logits, int64_t lstride, T* grad, int64_t gstride, int stage_bytes, int log_c,
-    RowArgs a) {
+    const T* logits, int64_t lstride, T* grad, int64_t gstride, int stage_bytes, int stages,
+    int log_c, RowArgs a) {
   using PK = PairPacket<T>;
   constexpr int VN = 16 / (int)sizeof(T);
   constexpr int NP = PK::N;
-  constexpr bool kKeep = !(TWO && sizeof(T) == 2);
   constexpr int kWarps = THREADS / 32;
   extern __shared__ __align__(128) unsigned char ring[];
-  float* picked = reinterpret_cast<float*>(ring + kStages * stage_bytes);  // [list]
-  __shared__ __align__(8) uint64_t full[kStages];
+  float* picked = reinterpret_cast<float*>(ring + stages * stage_bytes);  // [list]
+  __shared__ __align__(8) uint64_t full[kMaxStages];
   __shared__ __align__(8) uint64_t xbar[2];
   __shared__ __align__(16) float4 xch[2][8];
   __shared__ Stat wred[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = 1 << log_c, rank = (int)ptx::cluster_ctarank();
-  const int64_t first = blockIdx.x >> log_c, step = gridDim.x >> log_c;
+  const int n_rows = (int)a.n_rows, first = (int)(blockIdx.x >> log_c);
+  const int step = (int)(gridDim.x >> log_c);
   const bool loader = tid == THREADS - 32;  // the last warp's first lane starts the loads
 
   // A row's 16-byte packets and this CTA's share of them.
@@ -474,8 +485,8 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
     s.count = left < per ? (left < 0 ? 0 : left) : per;
     return s;
   };
-  auto issue = [&](int64_t row, int q) {  // loader: this CTA's slice of a row into stage q
-    if (row >= a.n_rows) return;
+  auto issue = [&](int row, int q) {  // loader: this CTA's slice of a row into stage q
+    if (row >= n_rows) return;
     const T* src = logits + row * lstride;
     const Slice s = slice_of(src);
     ptx::fence_proxy_async_smem();
@@ -488,7 +499,7 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
     }
   };
   if (tid == 0) {
-    for (int q = 0; q < kStages; ++q) ptx::mbar_init(&full[q], 1);
+    for (int q = 0; q < stages; ++q) ptx::mbar_init(&full[q], 1);
     ptx::mbar_init(&xbar[0], 1);
     ptx::mbar_init(&xbar[1], 1);
     ptx::fence_mbar_init();
@@ -496,30 +507,40 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
   if (C > 1) ptx::cluster_sync();
   else __syncthreads();
   if (loader)
-    for (int q = 0; q < kStages; ++q) issue(first + q * step, q);
+    for (int q = 0; q < stages; ++q) issue(first + q * step, q);
 
+  ptx::wait_for_previous_kernel();  // the logits are older; the rest is the teacher kernel's
   const float inv_n = 1.0f / count_valid(a);
   const float inv_t = a.inv_t;
   const float ct_row = inv_t * kLog2e;  // exponent of 2 per unit of logit
+  const bool same_slice = lstride % VN == 0;  // every row has the first row's offset
+  const bool lists = warp * 32 < a.list;      // this warp has listed elements to handle
   bool ok = true;
   double total = 0.0;
   int q = 0, phase = 0, xb = 0, xphase = 0;
   // What the row brings besides its logits is read one row ahead.
+  const int* next_id = a.ids + (int64_t)first * a.list + tid;
+  const float* next_p = a.probs + (int64_t)first * a.list + tid;
   int state = 0, my_id = -1;
   float my_p = 0.f, entropy = 0.f;
-  auto read_ahead = [&](int64_t row) {
-    if (row >= a.n_rows) return;
+  auto read_ahead = [&](int row) {
+    if (row >= n_rows) return;
     state = a.state[row];
     if (tid == THREADS - 1) entropy = a.entropy[row];
-    if (warp * 32 < a.list && tid < a.list) {
-      my_id = a.ids[row * a.list + tid];
-      my_p = a.probs[row * a.list + tid];
+    if (lists) {
+      if (tid < a.list) {
+        my_id = *next_id;
+        my_p = *next_p;
+      }
+      next_id += (int64_t)step * a.list;
+      next_p += (int64_t)step * a.list;
     }
   };
   read_ahead(first);
-  for (int64_t row = first; row < a.n_rows; row += step) {
-    const T* src = logits + row * lstride;
-    const Slice sl = slice_of(src);
+  const T* src = logits + first * lstride;
+  T* dst = grad + first * gstride;
+  Slice sl = slice_of(src);
+  for (int row = first; row < n_rows; row += step) {
     const int row_state = state, id = my_id;
     const float p_id = my_p, row_entropy = entropy;
     float xs = -INFINITY;  // an element outside the packets
@@ -535,10 +556,14 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
     PK p[KP];
 #pragma unroll
     for (int u = 0; u < KP; ++u) {
-      const int v = tid + u * THREADS;
-      constexpr uint32_t w = Pair<T>::kNegInf;
-      p[u].u = make_uint4(w, w, w, w);
-      if (v < sl.count) p[u].u = *reinterpret_cast<const uint4*>(stage + v * 16);
+      const uint4* at = reinterpret_cast<const uint4*>(stage) + tid + u * THREADS;
+      if ((u + 1) * THREADS <= sl.count) {
+        p[u].u = *at;
+      } else {
+        constexpr uint32_t w = Pair<T>::kNegInf;
+        p[u].u = make_uint4(w, w, w, w);
+        if (tid + u * THREADS < sl.count) p[u].u = *at;
+      }
     }
     // Listed elements of this slice: the same thread handles a listed place all through.
     auto mine = [&](int c) {  // whether element c is this CTA's
@@ -552,11 +577,15 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
       if (off >= (unsigned)(sl.packets * VN)) return Elt<T>::to_f(src[c]);
       return Elt<T>::to_f(reinterpret_cast<const T*>(stage)[(int)off - sl.start * VN]);
     };
-    const bool has = mine(id);
-    const float x_id = has ? value(id) : 0.f;
-    for (int j = tid + THREADS; j < a.list; j += THREADS) {
-      const int c = a.ids[row * a.list + j];
-      if (mine(c)) picked[j] = value(c);
+    bool has = false;
+    float x_id = 0.f;
+    if (lists) {
+      has = mine(id);
+      if (has) x_id = value(id);
+      for (int j = tid + THREADS; j < a.list; j += THREADS) {
+        const int c = a.ids[(int64_t)row * a.list + j];
+        if (mine(c)) picked[j] = value(c);
+      }
     }
     // This thread's maximum and exponentials.
     float my_m;
@@ -568,45 +597,45 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
       my_m = fmaxf(fmaxf(f.x, f.y), xs);
     }
     const float base = my_m == -INFINITY ? 0.f : my_m;
-    const float2 nb_t = make_float2(-base * ct_row, -base * ct_row);
-    const float2 nb_1 = make_float2(-base * kLog2e, -base * kLog2e);
-    auto exp_pair = [&](float2 x, float2& f, float2& f1) {
+    const float nb_t = -base * ct_row, nb_1 = -base * kLog2e;
+    auto exp_one = [&](float x, float& f, float& f1) {
       if constexpr (sizeof(T) == 2) {
-        const float2 t = __ffma2_rn(x, make_float2(ct_row, ct_row), nb_t);
-        f = make_float2(ex2f(t.x), ex2f(t.y));
-        if constexpr (TWO) {
-          const float2 t1 = __ffma2_rn(x, make_float2(kLog2e, kLog2e), nb_1);
-          f1 = make_float2(ex2f(t1.x), ex2f(t1.y));
-        }
+        f = ex2f(fmaf(x, ct_row, nb_t));
+        if constexpr (M == kTwo) f1 = ex2f(fmaf(x, kLog2e, nb_1));
       } else {
-        const float2 d = __fadd2_rn(x, make_float2(-base, -base));
-        f = exp2_of(TWO ? __fmul2_rn(d, make_float2(inv_t, inv_t)) : d);
-        if constexpr (TWO) f1 = exp2_of(d);
+        const float d = x - base;
+        f = exp2_of(d * inv_t);
+        if constexpr (M == kTwo) f1 = exp2_of(d);
       }
+      if constexpr (M == kSquare) f1 = f * f;
     };
-    float2 e[KP][kKeep ? NP : 1], e1[KP][kKeep && TWO ? NP : 1];
-    float2 es, es1 = make_float2(0.f, 0.f), z = make_float2(0.f, 0.f), z1 = z;
-    exp_pair(make_float2(xs, -INFINITY), es, es1);
-    z.x = es.x;
-    z1.x = es1.x;
+    float2 e[KEEP ? KP : 1][NP], e1[KEEP && M == kTwo ? KP : 1][NP];
+    float2 z = make_float2(0.f, 0.f), z1 = z;
+    if (xs_at >= 0) exp_one(xs, z.x, z1.x);
 #pragma unroll
     for (int u = 0; u < KP; ++u)
 #pragma unroll
       for (int k = 0; k < NP; ++k) {
-        float2 f, f1;
-        exp_pair(p[u].p[k].f(), f, f1);
-        z = __fadd2_rn(z, f);
-        if constexpr (TWO) z1 = __fadd2_rn(z1, f1);
-        if constexpr (kKeep) {
+        const float2 x = p[u].p[k].f();
+        float2 f, f1 = make_float2(0.f, 0.f);
+        exp_one(x.x, f.x, f1.x);
+        exp_one(x.y, f.y, f1.y);
+        z.x += f.x;
+        z.y += f.y;
+        if constexpr (M != kOne) {
+          z1.x += f1.x;
+          z1.y += f1.y;
+        }
+        if constexpr (KEEP) {
           e[u][k] = f;
-          if constexpr (TWO) e1[u][k] = f1;
+          if constexpr (M == kTwo) e1[u][k] = f1;
         }
       }
-    Stat st = join<T, TWO, 32>(Stat{my_m, z.x + z.y, TWO ? z1.x + z1.y : 0.f}, inv_t);
+    Stat st = join<T, M, 32>(Stat{my_m, z.x + z.y, M != kOne ? z1.x + z1.y : 0.f}, inv_t);
     if (lane == 0) wred[warp] = st;
     __syncthreads();  // the stage has been read by all
-    if (loader) issue(row + kStages * step, q);
-    if (C == 1 || warp == 0) st = join<T, TWO, kWarps>(wred[lane & (kWarps - 1)], inv_t);
+    if (loader) issue(row + stages * step, q);
+    if (C == 1 || warp == 0) st = join<T, M, kWarps>(wred[lane & (kWarps - 1)], inv_t);
     if (C > 1) {
       if (warp == 0) {
         if (lane == 0) ptx::mbar_arrive_expect_tx(&xbar[xb], (uint32_t)C * 16u);
@@ -620,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
       ok = ptx::mbar_wait(&xbar[xb], (uint32_t)xphase, ok ? (1u << 26) : 1u) && ok;
       const float4 f = xch[xb][lane & (C - 1)];
       const bool copy = (lane & 7) >= C;  // of a smaller cluster: counted once
-      st = join<T, TWO, 8>(Stat{f.x, copy ? 0.f : f.y, copy ? 0.f : f.z}, inv_t);
+      st = join<T, M, 8>(Stat{f.x, copy ? 0.f : f.y, copy ? 0.f : f.z}, inv_t);
     } else {
       read_ahead(row + step);
     }
@@ -628,56 +657,71 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
     const float hw = (row_state & kHard) ? a.hard_weight : 0.f;
     const float sw = (row_state & kSoft) ? 1.f - a.hard_weight : 0.f;
     const float ct = sw * a.temperature * a.loss_scale * inv_n, c1 = hw * a.loss_scale * inv_n;
-    const float kt = __fdividef(TWO ? ct : ct + c1, st.z), k1 = TWO ? __fdividef(c1, st.z1) : 0.f;
+    const float kt = __fdividef(M != kOne ? ct : ct + c1, st.z);
+    const float k1 = M != kOne ? __fdividef(c1, st.z1) : 0.f;
     const bool plain = row_state == kSkip || row_state == kBad;
     const float fill = row_state == kBad || !ok ? __int_as_float(0x7fc00000) : 0.f;
 
-    T* dst = grad + row * gstride;
-    T* out = dst + sl.head + sl.start * VN;
     if (grad) {
+      uint4* out = reinterpret_cast<uint4*>(dst + sl.head + sl.start * VN) + tid;
       if (plain) {
         PK o;
 #pragma unroll
         for (int k = 0; k < NP; ++k) o.p[k].set(make_float2(fill, fill));
-#pragma unroll
-        for (int u = 0; u < KP; ++u) {
-          const int v = tid + u * THREADS;
-          if (v < sl.count) __stcs(reinterpret_cast<uint4*>(out) + v, o.u);
-        }
+        for (int v = tid; v < sl.count; v += THREADS, out += THREADS) __stcs(out, o.u);
         if (xs_at >= 0) dst[xs_at] = Elt<T>::from_f(fill);
       } else {
+        // 16 bits: the factor k / z goes into the exponent.
+        const float ot = fmaf(-st.m, ct_row, __log2f(kt)), o1 = fmaf(-st.m, kLog2e, __log2f(k1));
+        auto dense = [&](float x) {
+          float g;
+          if constexpr (sizeof(T) == 2) {
+            if constexpr (M == kSquare) {  // k1 e^2 + kt e
+              const float f = ex2f(fmaf(x, ct_row, -st.m * ct_row));
+              g = f * fmaf(f, k1, kt);
+            } else {
+              g = ex2f(fmaf(x, ct_row, ot));
+              if constexpr (M == kTwo) g += ex2f(fmaf(x, kLog2e, o1));
+            }
+          } else {
+            const float d = x - st.m;
+            const float f = exp2_of(d * inv_t);
+            g = f * (M == kSquare ? fmaf(f, k1, kt) : kt);
+            if constexpr (M == kTwo) g = fmaf(exp2_of(d), k1, g);
+          }
+          return g;
+        };
         const bool none = my_m == -INFINITY;
-        // Without kept exponentials only the single element's were formed against base.
         // (A thread with nothing but -inf: 0, or NaN where the row's sum is.)
-        const float ft = (none ? 0.f : exp_of<T>((base - st.m) * inv_t)) * kt;
-        const float f1 = (none || !TWO ? 0.f : exp_of<T>(base - st.m)) * k1;
-        const float wt = kKeep ? ft : kt, w1 = kKeep ? f1 : k1;
-        const float2 ot = make_float2(-st.m * ct_row, -st.m * ct_row);
-        const float2 o1 = make_float2(-st.m * kLog2e, -st.m * kLog2e);
+        const float ft = KEEP ? (none ? 0.f : exp_of<T>((base - st.m) * inv_t)) * kt : 0.f;
+        const float f1 = KEEP && M != kOne ? (none ? 0.f : exp_of<T>(base - st.m)) * k1 : 0.f;
 #pragma unroll
         for (int u = 0; u < KP; ++u) {
-          const int v = tid + u * THREADS;
+          // Where the packet is converted anew, 32-bit copies kept from above would not fit.
+          if constexpr (!KEEP)
+            asm volatile("" : "+r"(p[u].u.x), "+r"(p[u].u.y), "+r"(p[u].u.z), "+r"(p[u].u.w));
           PK o;
 #pragma unroll
           for (int k = 0; k < NP; ++k) {
-            float2 f, g1 = make_float2(0.f, 0.f);
-            if constexpr (kKeep) {
-              f = e[u][k];
-              if constexpr (TWO) g1 = e1[u][k];
+            if constexpr (KEEP) {
+              const float2 f = e[u][k];
+              float2 g;
+              if constexpr (M == kSquare)
+                g = make_float2(f.x * fmaf(f.x, f1, ft), f.y * fmaf(f.y, f1, ft));
+              else
+                g = make_float2(f.x * ft, f.y * ft);
+              if constexpr (M == kTwo)
+                g = make_float2(fmaf(e1[u][k].x, f1, g.x), fmaf(e1[u][k].y, f1, g.y));
+              o.p[k].set(g);
             } else {
               const float2 x = p[u].p[k].f();
-              const float2 t = __ffma2_rn(x, make_float2(ct_row, ct_row), ot);
-              const float2 t1 = __ffma2_rn(x, make_float2(kLog2e, kLog2e), o1);
-              f = make_float2(ex2f(t.x), ex2f(t.y));
-              g1 = make_float2(ex2f(t1.x), ex2f(t1.y));
+              o.p[k].set(make_float2(dense(x.x), dense(x.y)));
             }
-            float2 g = __fmul2_rn(f, make_float2(wt, wt));
-            if constexpr (TWO) g = __ffma2_rn(g1, make_float2(w1, w1), g);
-            o.p[k].set(g);
           }
-          if (v < sl.count) __stcs(reinterpret_cast<uint4*>(out) + v, o.u);
+          if ((u + 1) * THREADS <= sl.count || tid + u * THREADS < sl.count)
+            __stcs(out + u * THREADS, o.u);
         }
-        if (xs_at >= 0) dst[xs_at] = Elt<T>::from_f(TWO ? fmaf(es.x, ft, es1.x * f1) : es.x * ft);
+        if (xs_at >= 0) dst[xs_at] = Elt<T>::from_f(dense(xs));
       }
     }
     __syncthreads();  // the listed places are written over the dense values
@@ -691,42 +735,51 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
       if (hw > 0.f && label) l -= hw * d;
       if (grad) {
         float g = kt * exp_of<T>(d * inv_t) - ct * pj;
-        if constexpr (TWO) g = fmaf(k1, exp_of<T>(d), g);
+        if constexpr (M != kOne) g = fmaf(k1, exp_of<T>(d), g);
         if (label) g -= c1;
         dst[c] = Elt<T>::from_f(g);
       }
     };
-    if (!plain && warp * 32 < a.list) {
+    if (!plain && lists) {
       if (has) listed(tid, id, x_id, p_id);
       for (int j = tid + THREADS; j < a.list; j += THREADS) {
-        const int c = a.ids[row * a.list + j];
-        if (mine(c)) listed(j, c, picked[j], a.probs[row * a.list + j]);
+        const int c = a.ids[(int64_t)row * a.list + j];
+        if (mine(c)) listed(j, c, picked[j], a.probs[(int64_t)row * a.list + j]);
       }
+      total += (double)l;
     }
     if (rank == 0 && tid == THREADS - 1) {
       if (plain) l = fill;
       else {
-        if (sw > 0.f) l += sw * a.temperature * a.temperature * (row_entropy + logf(st.z));
-        if (hw > 0.f) l += hw * logf(TWO ? st.z1 : st.z);
+        l = 0.f;
+        if (sw > 0.f) l = sw * a.temperature * a.temperature * (row_entropy + logf(st.z));
+        if (hw > 0.f) l += hw * logf(M != kOne ? st.z1 : st.z);
       }
+      total += (double)l;
     }
-    total += (double)l;
-    if (++q == kStages) {
+    if (++q == stages) {
       q = 0;
       phase ^= 1;
     }
     xphase ^= xb;
     xb ^= 1;
+    src += step * lstride;
+    dst += step * gstride;
+    if (!same_slice) sl = slice_of(src);
   }
   if (C > 1) ptx::cluster_sync();  // nobody's shared memory is written after its CTA is gone
   finish_loss(a, 1.0f / inv_n, total);
 }
 
-template <typename T, bool TWO, int THREADS, int KP, int MIN_CTAS>
+template <typename T, Mode M, bool KEEP, int THREADS, int KP, int MIN_CTAS>
 int launch_rows(const T* lp, int64_t ls, T* gp, int64_t gs, int log_c, int stage_bytes,
                 const RowArgs& a, cudaStream_t st) {
-  auto kern = distill_rows<T, TWO, THREADS, KP, MIN_CTAS>;
-  const int smem = kStages * stage_bytes + (a.list + 3) / 4 * 16;
+  auto kern = distill_rows<T, M, KEEP, THREADS, KP, MIN_CTAS>;
+  const int list_bytes = (a.list + 3) / 4 * 16;
+  // As many stages as leave room for MIN_CTAS on an SM (227 KB less 1 KB and the static part).
+  int stages = ((227 * 1024) / MIN_CTAS - 2048 - list_bytes) / stage_bytes;
+  stages = stages < 1 ? 1 : stages > kMaxStages ? kMaxStages : stages;
+  const int smem = stages * stage_bytes + list_bytes;
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   const int cluster = 1 << log_c;
   cudaLaunchConfig_t cfg = {};
@@ -734,7 +787,7 @@ int launch_rows(const T* lp, int64_t ls, T* gp, int64_t gs, int log_c, int stage
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -749,26 +802,36 @@ int launch_rows(const T* lp, int64_t ls, T* gp, int64_t gs, int log_c, int stage
   if (most * cluster > num_sms() * kMaxRowCtasPerSm) most = num_sms() * kMaxRowCtasPerSm / cluster;
   const int64_t clusters = a.n_rows < most ? a.n_rows : most;
   cfg.gridDim = dim3((unsigned)((clusters < 1 ? 1 : clusters) * cluster));
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, lp, ls, gp, gs, stage_bytes, log_c, a);
+  // The kernel may start, and load its first rows, while the teacher kernel ends.  Not so a
+  // grid of clusters that fills the GPU: placed among the teacher's last CTAs it finds no room
+  // for all its clusters at once, and the rest runs as a second wave (1186 against 717 us).
+  if (cluster == 1 || 2 * clusters <= most) {
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, lp, ls, gp, gs, stage_bytes, stages, log_c, a);
   if (e != cudaSuccess) return fail(FK_ERR_LAUNCH, "fk_distill(rows): %s", cudaGetErrorString(e));
   return launch_status("fk_distill(rows)");
 }
 
-template <typename T, bool TWO>
-int rows_two(const T* lp, int64_t ls, T* gp, int64_t gs, const RowArgs& a, cudaStream_t st) {
-  // Cluster: as many CTAs as a row needs for slices of at most 32 KB, more (down to 4 KB)
-  // while the rows are too few for the SMs.
+template <typename T, Mode M>
+int rows_mode(const T* lp, int64_t ls, T* gp, int64_t gs, const RowArgs& a, cudaStream_t st) {
+  // Cluster: as many CTAs as a row needs for slices of at most 32 KB (64 KB where 8 do not
+  // suffice), more (down to 8 KB) while the rows are too few for the SMs.  128 threads of 16
+  // packets and 4 such CTAs per SM measured best at 8192 x 128256 bf16: 717 us, against 809 with
+  // 256 threads and half the CTAs per row, 942 with 256 threads of 8 packets.
   const int64_t packets = (int64_t)a.n_cols * sizeof(T) / 16 + 1;
   int lc = 0;
   while (lc < 3 && packets > (int64_t)2048 << lc) ++lc;
   while (lc < 3 && (a.n_rows << lc) < num_sms() && (packets >> lc) > 512) ++lc;
   const int64_t per = (packets + ((int64_t)1 << lc) - 1) >> lc;
   const int bytes = (int)(per < 1 ? 16 : per * 16);
-  if (per <= 128) return launch_rows<T, TWO, 128, 1, 8>(lp, ls, gp, gs, lc, bytes, a, st);
-  if (per <= 512) return launch_rows<T, TWO, 128, 4, 8>(lp, ls, gp, gs, lc, bytes, a, st);
-  if (per <= 1024) return launch_rows<T, TWO, 128, 8, 4>(lp, ls, gp, gs, lc, bytes, a, st);
-  if (per <= 2048) return launch_rows<T, TWO, 256, 8, 2>(lp, ls, gp, gs, lc, bytes, a, st);
-  return launch_rows<T, TWO, 512, 8, 1>(lp, ls, gp, gs, lc, bytes, a, st);
+  constexpr bool keep = sizeof(T) == 4 && M != kTwo;
+  if (per <= 128) return launch_rows<T, M, true, 128, 1, 8>(lp, ls, gp, gs, lc, bytes, a, st);
+  if (per <= 512) return launch_rows<T, M, keep, 128, 4, 8>(lp, ls, gp, gs, lc, bytes, a, st);
+  if (per <= 2048) return launch_rows<T, M, keep, 128, 16, 4>(lp, ls, gp, gs, lc, bytes, a, st);
+  return launch_rows<T, M, keep, 256, 16, 2>(lp, ls, gp, gs, lc, bytes, a, st);
 }
 
 template <typename T>
@@ -780,8 +843,12 @@ int rows_t(const void* logits, int64_t ls, void* grad, int64_t gs, const RowArgs
   const bool same_offset = !gp || (apart % 16 == 0 && (ls - gs) * (int64_t)sizeof(T) % 16 == 0);
   const int64_t packets = (int64_t)a.n_cols * sizeof(T) / 16 + 1;
   if (same_offset && packets <= 8 * 4096) {
-    if (a.temperature == 1.0f) return rows_two<T, false>(lp, ls, gp, gs, a, st);
-    return rows_two<T, true>(lp, ls, gp, gs, a, st);
+    RowArgs b = a;
+    if (a.hard_weight == 1.f) b.temperature = b.inv_t = 1.f;  // the soft part has no weight
+    if (b.temperature == 1.f || a.hard_weight == 0.f)
+      return rows_mode<T, kOne>(lp, ls, gp, gs, b, st);
+    if (b.temperature == 2.f) return rows_mode<T, kSquare>(lp, ls, gp, gs, b, st);
+    return rows_mode<T, kTwo>(lp, ls, gp, gs, b, st);
   }
   const int64_t most = (int64_t)num_sms() * 8;
   const int grid = (int)(a.n_rows < most ? a.n_rows : most);
@@ -825,6 +892,7 @@ extern "C" int fk_distill(const void* logits, int64_t row_stride, void* grad,
                           void* workspace, size_t workspace_bytes, void* stream) {
   FK_CHECK_ARG(n_rows >= 0 && n_cols >= 1 && k >= 1, "fk_distill: bad shape");
   FK_CHECK_ARG(n_cols < ((int64_t)1 << 31) - 4096, "fk_distill: n_cols too large");
+  FK_CHECK_ARG(n_rows < ((int64_t)1 << 31) - 65536, "fk_distill: n_rows too large");
   if (k > fk::kMaxSlots)
     return fk::fail(FK_ERR_UNSUPPORTED, "fk_distill: k=%d exceeds %d", k, fk::kMaxSlots);
   FK_CHECK_ARG(fk::valid_dtype(dtype) && fk::valid_dtype(teacher_dtype), "fk_distill: bad dtype");
