@@ -7,7 +7,7 @@
 //   dloss/ds_c = 1/n * [(1-a) T (q_c - P_c) + a (softmax(s)_c - [c = y])],
 //   P_c = sum of the p_j whose id is c.
 //
-// The teacher's side of a row is small and is done first, by one warp per row: it leaves a
+// The teacher's side of a row is small and is done first, by a few lanes per row: it leaves a
 // list of (id, P) with every id once and the label's entry last, the row's sum p log p, and
 // partial counts of the rows that count (n).  The second kernel then needs every logit once
 // for the two sums and once for its gradient, and the gradient at the listed ids is computed
@@ -55,18 +55,44 @@ inline size_t ws_layout(void* base, int64_t n_rows, int k, Workspace* w) {
 }
 
 // ------------------------------------------------------------------ teacher -------------
-// Shared memory per warp: ids[k], p[k], and a hash table that finds ids standing twice.
-template <typename T>
+// Shared-memory words of a row; the rows of a warp lie 8 banks apart.
+__host__ __device__ inline int row_ints(int k, int log_table) {
+  return (2 * k + (1 << log_table) + 31) / 32 * 32 + 8;
+}
+
+// G lanes of a warp take a row.  Shared memory per row: ids[k], p[k], and a table that finds
+// ids standing twice: every slot writes its number at its id's hash and reads back whose number
+// is there.  Its own: the id is settled.  A slot of the same id: it stands twice.  Another id's:
+// the slot goes on to the next round, with another hash.  Slots of one id stay together until
+// one of them is settled and the others see it.  (Plain stores: inserting by atomicCAS took
+// 3.7 clocks a slot on an SM, 14 of the 18 us at 8192 rows of 64.)
+template <typename T, int G>
 __global__ void __launch_bounds__(kTeacherWarps * 32) distill_teacher(
-    const int64_t* __restrict__ idx, const T* __restrict__ top, int k, int table,
-    const int64_t* __restrict__ targets, int64_t ignore_index, int64_t n_rows, int64_t n_cols,
+    const int64_t* __restrict__ idx, const T* __restrict__ top, int k, int log_table,
+    const int64_t* __restrict__ targets, int64_t ignore_index, int n_rows, int64_t n_cols,
     float inv_t, Workspace ws) {
   extern __shared__ int smem[];
   __shared__ int valid_rows, bad_rows;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int* ids = smem + warp * (2 * k + table);
+  constexpr int kRows = kTeacherWarps * 32 / G;  // of a CTA at a time
+  const int at = threadIdx.x % G, slot = threadIdx.x / G;
+  int* ids = smem + slot * row_ints(k, log_table);
   float* p = reinterpret_cast<float*>(ids + k);
-  int* hash = ids + 2 * k;
+  int* table = ids + 2 * k;
+  auto group_max = [](float v) {
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  };
+  auto group_sum = [](float v) {
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  auto group_any = [&](bool b) {
+    const unsigned all = __ballot_sync(0xffffffffu, b);
+    const unsigned mine = (G == 32 ? 0xffffffffu : ((1u << (G & 31)) - 1u) << (threadIdx.x & 31 & ~(G - 1)));
+    return (all & mine) != 0;
+  };
   ptx::let_next_kernel_start();
   if (threadIdx.x == 0) {
     valid_rows = bad_rows = 0;
@@ -74,17 +100,20 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) distill_teacher(
   }
   __syncthreads();
   const int list = k + 1;
-  for (int64_t row = (int64_t)blockIdx.x * kTeacherWarps + warp; row < n_rows;
-       row += (int64_t)gridDim.x * kTeacherWarps) {
+  for (int base = blockIdx.x * kRows; base < n_rows; base += gridDim.x * kRows) {
+    const bool there = base + slot < n_rows;
+    const int row = there ? base + slot : n_rows - 1;  // idle groups go along on the last row
+    const int64_t* row_idx = idx + (int64_t)row * k;
+    const T* row_top = top + (int64_t)row * k;
     const int64_t y = targets ? targets[row] : -1;
     const bool ignored = targets && y == ignore_index;
     bool bad = targets && !ignored && (y < 0 || y >= n_cols);
     float m = -INFINITY;
     bool twice = false, nan = false;
 #pragma unroll 4
-    for (int j = lane; j < k; j += 32) {
-      const int64_t id = idx[row * k + j];
-      const float v = Elt<T>::to_f(top[row * k + j]);
+    for (int j = at; j < k; j += G) {
+      const int64_t id = row_idx[j];
+      const float v = Elt<T>::to_f(row_top[j]);
       const bool out = id >= n_cols;
       bad = bad || (out && !ignored);
       const int c = (id < 0 || out) ? -1 : (int)id;
@@ -95,36 +124,43 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) distill_teacher(
         nan = nan || v != v;
       }
     }
-    for (int i = lane; i < table; i += 32) hash[i] = -1;
+    m = group_max(m);
+    const bool held = m != -INFINITY || group_any(nan);
+    bad = group_any(bad);
     __syncwarp();
-    for (int j = lane; j < k; j += 32) {
-      const int c = ids[j];
-      if (c >= 0) {
-        unsigned at = ((unsigned)c * 2654435761u) & (unsigned)(table - 1);
-        for (;;) {  // at most k ids in a table of at least 2k places: a free one is found
-          const int old = atomicCAS(&hash[at], -1, c);
-          if (old == -1) break;
-          if (old == c) {
-            twice = true;
-            break;
-          }
-          at = (at + 1) & (unsigned)(table - 1);
-        }
+    float z = 0.f;
+    unsigned open = 0;  // this lane's slots that are not settled
+    for (int j = at, i = 0; j < k; j += G, ++i) {
+      if (ids[j] >= 0 && held) {
+        z += expf((p[j] - m) * inv_t);
+        open |= 1u << i;
+      } else {
+        ids[j] = -1;
       }
     }
-    bad = __any_sync(0xffffffffu, bad);
-    twice = __any_sync(0xffffffffu, twice);
-    m = warp_max(m);
-    float z = 0.f;
-    for (int j = lane; j < k; j += 32)
-      if (ids[j] >= 0) z += expf((p[j] - m) * inv_t);  // m = -inf: NaN, and the row has no teacher
-    z = warp_sum(z);
-    const bool held = m != -INFINITY || __any_sync(0xffffffffu, nan);
-    const float lz = logf(z), inv_z = 1.0f / z;
+    for (unsigned round = 0; __any_sync(0xffffffffu, open != 0); ++round) {
+      const unsigned factor = 2654435761u + round * 1640531526u;  // odd
+      for (unsigned o = open; o; o &= o - 1) {
+        const int j = at + (__ffs(o) - 1) * G;
+        table[(unsigned)ids[j] * factor >> (32 - log_table)] = j;
+      }
+      __syncwarp();
+      for (unsigned o = open; o; o &= o - 1) {
+        const int i = __ffs(o) - 1, j = at + i * G, c = ids[j];
+        const int there_j = table[(unsigned)c * factor >> (32 - log_table)];
+        const bool same = ids[there_j] == c;
+        if (same) open &= ~(1u << i);
+        twice = twice || (same && there_j != j);
+      }
+      __syncwarp();
+    }
+    twice = group_any(twice);
+    z = group_sum(z);
+    const float lz = logf(z), inv_z = held ? 1.0f / z : 0.f;
     float ent = 0.f;
-    for (int j = lane; j < k; j += 32) {
+    for (int j = at; j < k; j += G) {
       float pj = 0.f;
-      if (held && ids[j] >= 0) {
+      if (ids[j] >= 0) {
         const float d = (p[j] - m) * inv_t;
         pj = expf(d) * inv_z;
         if (pj > 0.f) ent = fmaf(pj, d - lz, ent);
@@ -132,15 +168,18 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) distill_teacher(
       }
       p[j] = pj;
     }
-    ent = warp_sum(ent);
+    ent = group_sum(ent);
     __syncwarp();
     int state = kSkip;
     if (!ignored && bad) state = kBad;
     else if (!ignored) state = (held ? kSoft : 0) | (targets ? kHard : 0);
+    const int label = (state & kHard) ? (int)y : -1;
     // The list: every id once, at its first slot, with the sum of its probabilities; the
     // label's at the end.
     float py = 0.f;
-    for (int j = lane; j < k; j += 32) {
+    int* out_ids = ws.ids + (int64_t)row * list;
+    float* out_probs = ws.probs + (int64_t)row * list;
+    for (int j = at; j < k; j += G) {
       int c = ids[j];
       float pj = p[j];
       if (twice && c >= 0) {
@@ -153,18 +192,19 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) distill_teacher(
           }
         if (first != j) c = -1;
       }
-      if ((state & kHard) && c == (int)y && c >= 0) {
+      if (c >= 0 && c == label) {
         py += pj;
         c = -1;
       }
-      if (!held) c = -1;
-      ws.ids[row * list + j] = c;
-      ws.probs[row * list + j] = c >= 0 ? pj : 0.f;
+      if (there) {
+        out_ids[j] = c;
+        out_probs[j] = c >= 0 ? pj : 0.f;
+      }
     }
-    py = warp_sum(py);
-    if (lane == 0) {
-      ws.ids[row * list + k] = (state & kHard) ? (int)y : -1;
-      ws.probs[row * list + k] = py;
+    py = group_sum(py);
+    if (at == 0 && there) {
+      out_ids[k] = label;
+      out_probs[k] = py;
       ws.entropy[row] = ent;
       ws.state[row] = state;
       if (state != kSkip) atomicAdd(&valid_rows, 1);
@@ -860,15 +900,20 @@ template <typename T>
 int teacher_t(const int64_t* idx, const void* top, int k, const int64_t* targets,
               int64_t ignore_index, int64_t n_rows, int64_t n_cols, float inv_t,
               const Workspace& ws, int* ctas, cudaStream_t st) {
-  int table = 32;
-  while (table < 2 * k) table *= 2;
-  const int smem = kTeacherWarps * (2 * k + table) * 4;
-  const int64_t want = (n_rows + kTeacherWarps - 1) / kTeacherWarps;
+  int log_table = 5;
+  while ((1 << log_table) < 2 * k) ++log_table;
+  // Many short rows: 8 lanes a row, so that the reductions of 4 rows are one instruction.  Few
+  // or long ones: a warp a row.
+  const bool narrow = n_rows >= 4096 && k <= 128;
+  const int rows = kTeacherWarps * (narrow ? 4 : 1);
+  const int smem = rows * row_ints(k, log_table) * 4;
+  const int64_t want = (n_rows + rows - 1) / rows;
   *ctas = (int)(want < 1 ? 1 : want > kTeacherCtas ? kTeacherCtas : want);
-  auto kern = distill_teacher<T>;
+  auto kern = narrow ? distill_teacher<T, 8> : distill_teacher<T, 32>;
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  kern<<<*ctas, kTeacherWarps * 32, smem, st>>>(idx, static_cast<const T*>(top), k, table, targets,
-                                                ignore_index, n_rows, n_cols, inv_t, ws);
+  kern<<<*ctas, kTeacherWarps * 32, smem, st>>>(idx, static_cast<const T*>(top), k, log_table,
+                                                targets, ignore_index, (int)n_rows, n_cols, inv_t,
+                                                ws);
   return launch_status("fk_distill(teacher)");
 }
 
