@@ -144,7 +144,8 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 
 def stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """Handle of the current stream of ``t``'s device."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
@@ -215,19 +216,26 @@ def on_device(t: torch.Tensor):
     return _NO_SWITCH if i == torch.cuda.current_device() else torch.cuda.device(i)
 
 
-def rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
-    """``t`` as [rows, cols] with unit stride along a row and rows that do not overlap
-    (a view where there is one)."""
+def rows_of(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int]:
+    """``t`` seen as rows of ``cols`` elements with unit stride, and the rows' stride in
+    elements: a tensor to read from (t itself, a view or a copy)."""
+    if t.is_contiguous():
+        return t, cols
     t = t.reshape(-1, cols)
-    if t.shape[0] > 1 and t.stride(0) < cols or cols > 1 and t.stride(1) != 1:
-        t = t.contiguous()
-    return t
+    if cols > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < cols:
+        return t.contiguous(), cols
+    return t, max(t.stride(0), cols)  # a tensor of one row may report any stride
 
 
-def row_stride(t: torch.Tensor) -> int:
-    """Row stride of a [rows, cols] tensor from rows_of, in elements (a tensor of one row
-    may report any stride)."""
-    return max(t.stride(0), t.shape[1])
+def once_differentiable(fn):
+    """torch's once_differentiable, without its cost where no graph of the backward pass is
+    wanted (grad mode is off there)."""
+    guarded = torch.autograd.function.once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+
+    return backward
 
 
 def hand_over_gradient(ctx, grad_output: torch.Tensor) -> torch.Tensor:
@@ -239,12 +247,13 @@ def hand_over_gradient(ctx, grad_output: torch.Tensor) -> torch.Tensor:
         raise RuntimeError("the gradient of this loss was handed over in its first backward "
                            "pass: compute the loss again for another one")
     ctx.grad = None
-    go = grad_output.to(torch.float32)
+    go = grad_output if grad_output.dtype == torch.float32 else grad_output.to(torch.float32)
     if ctx.loss_scale != 1.0:
         go = go / ctx.loss_scale
+    rows, cols = grad.shape
     with on_device(grad):
-        call("fk_ce_bwd_scale", grad.data_ptr(), row_stride(grad), grad.shape[0], grad.shape[1],
-             go.data_ptr(), dtype_code(grad.dtype), stream_of(grad))
+        call("fk_ce_bwd_scale", grad.data_ptr(), max(grad.stride(0), cols), rows, cols,
+             go.data_ptr(), _DTYPE_CODES[grad.dtype], stream_of(grad))
     return grad.detach()
 
 

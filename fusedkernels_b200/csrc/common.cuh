@@ -9,6 +9,8 @@
 #include <stdio.h>
 #include <stdarg.h>
 
+#include <atomic>
+
 #include "../../include/fkb200.h"
 
 namespace fk {
@@ -23,6 +25,20 @@ int num_sms();                         // SM count of the current device (cached
   do {                                                            \
     if (!(cond)) return ::fk::fail(FK_ERR_INVALID_ARG, __VA_ARGS__); \
   } while (0)
+
+// Lets KERNEL take as much dynamic shared memory as the current device has for a CTA beside
+// `static_bytes` of static shared memory (asked for once per device; a launch still names what
+// it uses).
+template <auto KERNEL>
+inline void allow_shared_memory(int static_bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = -1;
+  if (dev >= 0 && (done.load(std::memory_order_relaxed) >> dev & 1)) return;
+  cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       227 * 1024 - static_bytes);
+  if (dev >= 0) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+}
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -814,13 +814,13 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
 template <typename T, Mode M, bool KEEP, int THREADS, int KP, int MIN_CTAS>
 int launch_rows(const T* lp, int64_t ls, T* gp, int64_t gs, int log_c, int stage_bytes,
                 const RowArgs& a, cudaStream_t st) {
-  auto kern = distill_rows<T, M, KEEP, THREADS, KP, MIN_CTAS>;
+  constexpr auto kern = distill_rows<T, M, KEEP, THREADS, KP, MIN_CTAS>;
   const int list_bytes = (a.list + 3) / 4 * 16;
   // As many stages as leave room for MIN_CTAS on an SM (227 KB less 1 KB and the static part).
   int stages = ((227 * 1024) / MIN_CTAS - 2048 - list_bytes) / stage_bytes;
   stages = stages < 1 ? 1 : stages > kMaxStages ? kMaxStages : stages;
   const int smem = stages * stage_bytes + list_bytes;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  allow_shared_memory<kern>(2048);
   const int cluster = 1 << log_c;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)cluster);
@@ -834,11 +834,20 @@ int launch_rows(const T* lp, int64_t ls, T* gp, int64_t gs, int log_c, int stage
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   // The grid is what the GPU holds at once (clusters of 8 do not fill every SM).
-  int most = 0;
-  if (cudaOccupancyMaxActiveClusters(&most, kern, &cfg) != cudaSuccess || most < 1) {
-    cudaGetLastError();
-    most = 1;
+  // The last answer of this thread is kept: it depends on the device and these sizes alone.
+  static thread_local int asked_dev = -1, asked_smem, asked_cluster, answer;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+  if (asked_dev != dev || asked_smem != smem || asked_cluster != cluster) {
+    if (cudaOccupancyMaxActiveClusters(&answer, kern, &cfg) != cudaSuccess || answer < 1) {
+      cudaGetLastError();
+      answer = 1;
+    }
+    asked_dev = dev;
+    asked_smem = smem;
+    asked_cluster = cluster;
   }
+  int most = answer;
   if (most * cluster > num_sms() * kMaxRowCtasPerSm) most = num_sms() * kMaxRowCtasPerSm / cluster;
   const int64_t clusters = a.n_rows < most ? a.n_rows : most;
   cfg.gridDim = dim3((unsigned)((clusters < 1 ? 1 : clusters) * cluster));
@@ -904,16 +913,19 @@ int teacher_t(const int64_t* idx, const void* top, int k, const int64_t* targets
   while ((1 << log_table) < 2 * k) ++log_table;
   // Many short rows: 8 lanes a row, so that the reductions of 4 rows are one instruction.  Few
   // or long ones: a warp a row.
-  const bool narrow = n_rows >= 4096 && k <= 128;
+  const bool narrow = n_rows >= 4096 && k <= 64;
   const int rows = kTeacherWarps * (narrow ? 4 : 1);
   const int smem = rows * row_ints(k, log_table) * 4;
   const int64_t want = (n_rows + rows - 1) / rows;
   *ctas = (int)(want < 1 ? 1 : want > kTeacherCtas ? kTeacherCtas : want);
-  auto kern = narrow ? distill_teacher<T, 8> : distill_teacher<T, 32>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  kern<<<*ctas, kTeacherWarps * 32, smem, st>>>(idx, static_cast<const T*>(top), k, log_table,
-                                                targets, ignore_index, (int)n_rows, n_cols, inv_t,
-                                                ws);
+  auto launch = [&](auto kern) {
+    kern<<<*ctas, kTeacherWarps * 32, smem, st>>>(idx, static_cast<const T*>(top), k, log_table,
+                                                  targets, ignore_index, (int)n_rows, n_cols,
+                                                  inv_t, ws);
+  };
+  allow_shared_memory<distill_teacher<T, 32>>(1024);  // 8 lanes a row stay below 48 KB
+  if (narrow) launch(distill_teacher<T, 8>);
+  else launch(distill_teacher<T, 32>);
   return launch_status("fk_distill(teacher)");
 }
 

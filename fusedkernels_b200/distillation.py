@@ -12,7 +12,6 @@ logits.  Over the used slots of a row (id >= 0), with temperature T and s the st
 gradient written once, as ``fused_cross_entropy`` does; the two losses share that pass.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -22,42 +21,44 @@ _last_err = None
 
 class _FusedDistillation(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, teacher_idx, teacher_logits, targets, temperature, hard_weight,
-                ignore_index, inplace_grad, loss_scale, want_grad):
+    def forward(ctx, logits, args):
         global _last_err
+        (teacher_idx, teacher_logits, targets, temperature, hard_weight, ignore_index,
+         inplace_grad, loss_scale, want_grad) = args
         n_rows, n_cols = logits.shape
         dev = logits.device
-        x = logits
-        if n_cols > 1 and x.stride(1) != 1 or n_rows > 1 and x.stride(0) < n_cols:
-            x = x.contiguous()
+        x, stride = _lib.rows_of(logits, n_cols)
         idx = teacher_idx.to(torch.int64).contiguous()
         top = teacher_logits.contiguous()
         if targets is not None:
             targets = targets.to(torch.int64).contiguous()
-        grad = None
+        grad, grad_stride = None, n_cols
         if want_grad:
-            grad = x if inplace_grad else torch.empty(n_rows, n_cols, dtype=x.dtype, device=dev)
+            if inplace_grad:
+                grad, grad_stride = x, stride
+            else:
+                grad = torch.empty((n_rows, n_cols), dtype=x.dtype, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev)
         err = torch.empty(1, dtype=torch.int32, device=dev)
         k = idx.shape[1]
-        ws = torch.empty(_lib.workspace_bytes("fk_distill_workspace_size", dev, n_rows, k),
-                         dtype=torch.uint8, device=dev)
+        size = _lib.workspace_bytes("fk_distill_workspace_size", dev, n_rows, k)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
         with _lib.on_device(logits):
-            _lib.call("fk_distill", x.data_ptr(), _lib.row_stride(x), _lib.ptr(grad),
-                      0 if grad is None else _lib.row_stride(grad), idx.data_ptr(),
-                      top.data_ptr(), _lib.dtype_code(top.dtype), k, _lib.ptr(targets), n_rows,
-                      n_cols, ignore_index, temperature, hard_weight, loss_scale,
-                      _lib.dtype_code(x.dtype), loss.data_ptr(), err.data_ptr(), ws.data_ptr(),
-                      ws.numel(), _lib.stream_of(logits))
+            _lib.call("fk_distill", x.data_ptr(), stride, _lib.ptr(grad), grad_stride,
+                      idx.data_ptr(), top.data_ptr(), _lib.dtype_code(top.dtype), k,
+                      _lib.ptr(targets), n_rows, n_cols, ignore_index, temperature, hard_weight,
+                      loss_scale, _lib.dtype_code(x.dtype), loss.data_ptr(), err.data_ptr(),
+                      ws.data_ptr(), size, _lib.stream_of(logits))
         _last_err = err
-        ctx.grad = grad
-        ctx.loss_scale = loss_scale
+        if want_grad:
+            ctx.grad = grad
+            ctx.loss_scale = loss_scale
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, grad_output):
-        return (_lib.hand_over_gradient(ctx, grad_output),) + (None,) * 9
+        return _lib.hand_over_gradient(ctx, grad_output), None
 
 
 def fused_distillation_loss(logits: torch.Tensor, teacher_idx: torch.Tensor,
@@ -96,10 +97,11 @@ def fused_distillation_loss(logits: torch.Tensor, teacher_idx: torch.Tensor,
         assert targets.shape == (n_rows,) and targets.device == logits.device
         assert not targets.is_floating_point()
     assert temperature > 0.0 and 0.0 <= hard_weight <= 1.0 and loss_scale != 0.0
-    return _FusedDistillation.apply(logits, teacher_idx, teacher_logits, targets,
-                                    float(temperature), float(hard_weight), int(ignore_index),
-                                    inplace_grad, float(loss_scale),
-                                    torch.is_grad_enabled() and logits.requires_grad)
+    want_grad = torch.is_grad_enabled() and logits.requires_grad
+    return _FusedDistillation.apply(logits, (teacher_idx, teacher_logits, targets,
+                                             float(temperature), float(hard_weight),
+                                             int(ignore_index), inplace_grad, float(loss_scale),
+                                             want_grad))
 
 
 def last_distillation_error() -> int:

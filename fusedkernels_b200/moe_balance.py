@@ -13,7 +13,6 @@ its gradient with the loss, so the backward pass launches nothing but the check 
 grad_output.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .moe_routing_v2 import MAX_EXPERTS
@@ -21,33 +20,34 @@ from .moe_routing_v2 import MAX_EXPERTS
 
 class _FusedMoEBalanceLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, topk_idx, token_mask, z_coef, loss_scale, want_grad):
+    def forward(ctx, logits, args):
+        topk_idx, token_mask, z_coef, loss_scale, want_grad = args
         n_rows, n_experts = logits.shape
         dev = logits.device
-        x = logits
-        if n_experts > 1 and x.stride(1) != 1 or n_rows > 1 and x.stride(0) < n_experts:
-            x = x.contiguous()
+        x, stride = _lib.rows_of(logits, n_experts)
         idx = topk_idx.to(torch.int64).contiguous()
         mask = None if token_mask is None else token_mask.contiguous()
-        grad = torch.empty(n_rows, n_experts, dtype=x.dtype, device=dev) if want_grad else None
+        grad = torch.empty((n_rows, n_experts), dtype=x.dtype, device=dev) if want_grad else None
         counts = torch.empty(n_experts, dtype=torch.int64, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        ws = torch.empty(_lib.workspace_bytes("fk_moe_balance_workspace_size", dev),
-                         dtype=torch.uint8, device=dev)
+        size = _lib.workspace_bytes("fk_moe_balance_workspace_size", dev)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
         with _lib.on_device(logits):
-            _lib.call("fk_moe_balance", x.data_ptr(), _lib.row_stride(x), idx.data_ptr(),
-                      _lib.ptr(mask), n_rows, n_experts, idx.shape[1], z_coef, loss_scale,
-                      _lib.ptr(grad), counts.data_ptr(), loss.data_ptr(), ws.data_ptr(),
-                      ws.numel(), _lib.dtype_code(x.dtype), _lib.stream_of(logits))
-        ctx.grad = grad
-        ctx.loss_scale = loss_scale
-        ctx.mark_non_differentiable(counts)
+            _lib.call("fk_moe_balance", x.data_ptr(), stride, idx.data_ptr(), _lib.ptr(mask),
+                      n_rows, n_experts, idx.shape[1], z_coef, loss_scale, _lib.ptr(grad),
+                      counts.data_ptr(), loss.data_ptr(), ws.data_ptr(), size,
+                      _lib.dtype_code(x.dtype), _lib.stream_of(logits))
+        if want_grad:
+            ctx.grad = grad
+            ctx.loss_scale = loss_scale
+            ctx.set_materialize_grads(False)
+            ctx.mark_non_differentiable(counts)
         return loss, counts
 
     @staticmethod
-    @once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, grad_output, _counts):
-        return _lib.hand_over_gradient(ctx, grad_output), None, None, None, None, None
+        return None if grad_output is None else _lib.hand_over_gradient(ctx, grad_output), None
 
 
 def fused_moe_balance_loss(router_logits: torch.Tensor, topk_idx: torch.Tensor,
@@ -76,6 +76,6 @@ def fused_moe_balance_loss(router_logits: torch.Tensor, topk_idx: torch.Tensor,
         assert token_mask.shape == (n_rows,) and token_mask.dtype == torch.bool
         assert token_mask.device == router_logits.device
     assert loss_scale != 0.0
-    return _FusedMoEBalanceLoss.apply(router_logits, topk_idx, token_mask, float(z_coef),
-                                      float(loss_scale),
-                                      torch.is_grad_enabled() and router_logits.requires_grad)
+    want_grad = torch.is_grad_enabled() and router_logits.requires_grad
+    return _FusedMoEBalanceLoss.apply(router_logits, (topk_idx, token_mask, float(z_coef),
+                                                      float(loss_scale), want_grad))

@@ -9,7 +9,6 @@ device in a fixed order (per-CTA partial rows + a column reduce), replacing the
 """
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -68,41 +67,44 @@ _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 def _check_add_norm(x, residual, weight):
     assert x.is_cuda and weight.is_cuda and x.ndim >= 1
     assert x.dtype in _FLOATS and weight.dtype in _FLOATS, "fp32, fp16 or bf16 tensors"
-    assert weight.numel() == x.shape[-1] and x.shape[-1] >= 1
+    assert weight.numel() == x.shape[-1] >= 1
     assert weight.device == x.device
     if residual is not None:
         assert residual.shape == x.shape, "residual and x have one shape (nothing is broadcast)"
         assert residual.device == x.device
-        assert residual.dtype in (x.dtype, torch.float32), "the residual has x's dtype or fp32"
+        assert residual.dtype == x.dtype or residual.dtype == torch.float32, \
+            "the residual has x's dtype or fp32"
 
 
 class _FusedAddRMSNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps, save):
-        ctx.set_materialize_grads(False)
         n_cols = x.shape[-1]
-        x2, r2 = _lib.rows_of(x, n_cols), _lib.rows_of(residual, n_cols)
-        n_rows = x2.shape[0]
+        n_rows = x.numel() // n_cols
+        x2, xs = _lib.rows_of(x, n_cols)
+        r2, rs = _lib.rows_of(residual, n_cols)
         w = weight.contiguous()
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-        rstd = torch.empty(n_rows, dtype=torch.float32, device=x.device) if save else None
+        dev = x.device
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
+        rstd = torch.empty(n_rows, dtype=torch.float32, device=dev) if save else None
         with _lib.on_device(x):
-            _lib.call("fk_add_rmsnorm_fwd", x2.data_ptr(), _lib.row_stride(x2), r2.data_ptr(),
-                      _lib.row_stride(r2), _lib.dtype_code(r2.dtype), w.data_ptr(),
-                      _lib.dtype_code(w.dtype), y.data_ptr(), h.data_ptr(), _lib.ptr(rstd),
-                      n_rows, n_cols, float(eps), _lib.dtype_code(x2.dtype), _lib.stream_of(x))
+            _lib.call("fk_add_rmsnorm_fwd", x2.data_ptr(), xs, r2.data_ptr(), rs,
+                      _lib.dtype_code(h.dtype), w.data_ptr(), _lib.dtype_code(w.dtype),
+                      y.data_ptr(), h.data_ptr(), _lib.ptr(rstd), n_rows, n_cols, eps,
+                      _lib.dtype_code(y.dtype), _lib.stream_of(x))
         if save:
+            ctx.set_materialize_grads(False)
             ctx.save_for_backward(h, w, rstd)
             ctx.x_dtype = x.dtype
             ctx.weight_shape = weight.shape
         return y, h
 
     @staticmethod
-    @once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dy, dh):
         h, w, rstd = ctx.saved_tensors
-        shape, n_cols = h.shape, h.shape[-1]
+        n_cols = h.shape[-1]
         need_x, need_r, need_w = ctx.needs_input_grad[:3]
         if dy is None:  # only the sum was used: its gradient passes through
             if dh is None:
@@ -110,22 +112,21 @@ class _FusedAddRMSNormFn(torch.autograd.Function):
             return (dh.to(ctx.x_dtype) if need_x else None, dh if need_r else None,
                     torch.zeros(ctx.weight_shape, dtype=w.dtype, device=w.device)
                     if need_w else None, None, None)
-        dy2 = _lib.rows_of(dy, n_cols)
-        dh2 = None if dh is None else _lib.rows_of(dh, n_cols)
-        n_rows = dy2.shape[0]
-        dx = torch.empty(shape, dtype=ctx.x_dtype, device=h.device)
+        dev = h.device
+        dy2, dys = _lib.rows_of(dy, n_cols)
+        dh2, dhs = (None, 0) if dh is None else _lib.rows_of(dh, n_cols)
+        n_rows = h.numel() // n_cols
+        dx = torch.empty(h.shape, dtype=ctx.x_dtype, device=dev)
         dr = dx if h.dtype == ctx.x_dtype else torch.empty_like(h)
-        dw = torch.empty(ctx.weight_shape, dtype=w.dtype, device=h.device)
-        ws = torch.empty(max(_lib.workspace_bytes("fk_add_rmsnorm_bwd_workspace_size", h.device,
-                                                  n_rows, n_cols), 16),
-                         dtype=torch.uint8, device=h.device)
+        dw = torch.empty(ctx.weight_shape, dtype=w.dtype, device=dev)
+        size = _lib.workspace_bytes("fk_add_rmsnorm_bwd_workspace_size", dev, n_rows, n_cols)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
         with _lib.on_device(h):
-            _lib.call("fk_add_rmsnorm_bwd", dy2.data_ptr(), _lib.row_stride(dy2), _lib.ptr(dh2),
-                      0 if dh2 is None else _lib.row_stride(dh2), h.data_ptr(),
+            _lib.call("fk_add_rmsnorm_bwd", dy2.data_ptr(), dys, _lib.ptr(dh2), dhs, h.data_ptr(),
                       _lib.dtype_code(h.dtype), w.data_ptr(), _lib.dtype_code(w.dtype),
                       rstd.data_ptr(), dx.data_ptr(), None if dr is dx else dr.data_ptr(),
-                      dw.data_ptr(), ws.data_ptr(), ws.numel(), n_rows, n_cols,
-                      _lib.dtype_code(ctx.x_dtype), _lib.stream_of(h))
+                      dw.data_ptr(), ws.data_ptr(), size, n_rows, n_cols,
+                      _lib.dtype_code(dx.dtype), _lib.stream_of(h))
         return dx if need_x else None, dr if need_r else None, dw if need_w else None, None, None
 
 
@@ -141,7 +142,7 @@ def fused_add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Te
     _check_add_norm(x, residual, weight)
     save = torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or
                                         weight.requires_grad)
-    return _FusedAddRMSNormFn.apply(x, residual, weight, eps, save)
+    return _FusedAddRMSNormFn.apply(x, residual, weight, float(eps), save)
 
 
 def fused_add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None,
@@ -162,23 +163,22 @@ def fused_add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None,
                  (residual is not None and residual.requires_grad))), \
         "fused_add_rms_norm_quant has no gradient: call it under torch.no_grad()"
     n_cols = x.shape[-1]
-    x2 = _lib.rows_of(x, n_cols)
-    n_rows = x2.shape[0]
+    n_rows = x.numel() // n_cols
+    x2, xs = _lib.rows_of(x, n_cols)
     w = weight.contiguous()
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    dev = x.device
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
     groups = 1 if block is None else -(-n_cols // block)
-    scales = torch.empty(*x.shape[:-1], groups, dtype=torch.float32, device=x.device)
-    r2, h = None, x
+    scales = torch.empty((*x.shape[:-1], groups), dtype=torch.float32, device=dev)
+    r2, rs, h = None, 0, x
     if residual is not None:
-        r2 = _lib.rows_of(residual, n_cols)
-        h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+        r2, rs = _lib.rows_of(residual, n_cols)
+        h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
     with _lib.on_device(x):
-        _lib.call("fk_add_rmsnorm_quant", x2.data_ptr(), _lib.row_stride(x2), _lib.ptr(r2),
-                  0 if r2 is None else _lib.row_stride(r2),
-                  _lib.dtype_code(x2.dtype if r2 is None else r2.dtype), w.data_ptr(),
-                  _lib.dtype_code(w.dtype), q.data_ptr(), scales.data_ptr(),
-                  None if r2 is None else h.data_ptr(), n_rows, n_cols, block or 0, float(eps),
-                  _lib.dtype_code(x2.dtype), _lib.stream_of(x))
+        _lib.call("fk_add_rmsnorm_quant", x2.data_ptr(), xs, _lib.ptr(r2), rs,
+                  _lib.dtype_code(h.dtype), w.data_ptr(), _lib.dtype_code(w.dtype), q.data_ptr(),
+                  scales.data_ptr(), None if r2 is None else h.data_ptr(), n_rows, n_cols,
+                  block or 0, float(eps), _lib.dtype_code(x.dtype), _lib.stream_of(x))
     return q, scales, h
 
 
