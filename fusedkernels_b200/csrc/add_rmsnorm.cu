@@ -46,6 +46,242 @@ __device__ __forceinline__ float block_max(float v, float* red) {
   return m;
 }
 
+// ------------------------------------------------------------------ 16-byte chunks ------
+// A chunk is 16 bytes of x (VN elements) and the same elements of the residual: one 16-byte
+// load, or two where the residual is fp32 beside 16-bit x.
+template <typename R, int VN>
+struct Chunk {
+  static constexpr int N16 = VN * (int)sizeof(R) / 16;
+  union {
+    uint4 u[N16];
+    R e[VN];
+  };
+  __device__ __forceinline__ Chunk() {}
+  __device__ __forceinline__ void load(const R* p) {
+#pragma unroll
+    for (int i = 0; i < N16; ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void store(R* p) const {
+#pragma unroll
+    for (int i = 0; i < N16; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, u[i]);
+  }
+};
+
+// VN weights from column c on (a multiple of VN), in fp32; they stay in L1 from row to row.
+template <int VN>
+__device__ __forceinline__ void load_weights(const void* w, int wd, int c, float (&out)[VN]) {
+  if (wd == FK_F32) {
+#pragma unroll
+    for (int i = 0; i < VN; i += 4) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(w) + c + i));
+      out[i] = f.x;
+      out[i + 1] = f.y;
+      out[i + 2] = f.z;
+      out[i + 3] = f.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < VN; i += 4) {
+    const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(w) + c + i));
+    const uint32_t h[2] = {u.x, u.y};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const unsigned short b = (unsigned short)(h[k >> 1] >> (16 * (k & 1)));
+      out[i + k] = wd == FK_F16 ? __half2float(__ushort_as_half(b))
+                                : __bfloat162float(__ushort_as_bfloat16(b));
+    }
+  }
+}
+
+// Sum (or maximum) over the TPR threads that share a row; all of them get it.  Groups of more
+// than a warp are whole CTAs.
+template <int TPR, bool MAX>
+__device__ __forceinline__ float row_reduce(float v, float* red) {
+#pragma unroll
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) {
+    const float b = __shfl_xor_sync(0xffffffffu, v, o);
+    v = MAX ? fmaxf(v, b) : v + b;
+  }
+  if constexpr (TPR > 32) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    v = red[lane % (TPR / 32)];  // fixed order: deterministic
+#pragma unroll
+    for (int o = TPR / 64; o > 0; o >>= 1) {
+      const float b = __shfl_xor_sync(0xffffffffu, v, o);
+      v = MAX ? fmaxf(v, b) : v + b;
+    }
+  }
+  return v;
+}
+
+constexpr int fwd_groups(int tpr) { return tpr <= 32 ? 256 / tpr : 1; }
+
+// Forward, and with QUANT the 8-bit form (BLOCK: a scale per 128 columns, else per row).  TPR
+// threads take a row, thread t its chunks t, t + TPR, ...: every load of the row is in flight
+// before the first is used, the sum h stays in registers, and as the rows are independent the
+// SM hides one CTA's reduction under the others' loads.
+template <typename T, typename R, int TPR, int CPT, bool QUANT, bool BLOCK>
+__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR) add_rmsnorm_rows(
+    const T* __restrict__ x, int64_t xs, const R* __restrict__ r, int64_t rs,
+    const void* __restrict__ w, int wd, T* __restrict__ y, uint8_t* __restrict__ q,
+    float* __restrict__ scales, R* __restrict__ h, float* __restrict__ rstd, int64_t rows,
+    int cols, float eps) {
+  constexpr int VN = 16 / (int)sizeof(T);
+  __shared__ float red[2][32];
+  const int t = threadIdx.x % TPR;
+  const int64_t row0 = (int64_t)blockIdx.x * fwd_groups(TPR) + threadIdx.x / TPR;
+  const bool there = TPR > 32 || row0 < rows;
+  const int64_t row = there ? row0 : rows - 1;  // idle groups go along on the last row
+  const int chunks = cols / VN;
+  Chunk<T, VN> xv[CPT];
+  Chunk<R, VN> hv[CPT];
+#pragma unroll
+  for (int u = 0; u < CPT; ++u) {
+    const int c = t + u * TPR;
+    if (c < chunks) {
+      xv[u].load(x + row * xs + c * VN);
+      if (r) hv[u].load(r + row * rs + c * VN);
+    }
+  }
+  float wv[CPT][VN];
+#pragma unroll
+  for (int u = 0; u < CPT; ++u) {
+    const int c = t + u * TPR;
+    if (c < chunks) load_weights<VN>(w, wd, c * VN, wv[u]);
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int u = 0; u < CPT; ++u) {
+    const int c = t + u * TPR;
+    if (c < chunks) {
+#pragma unroll
+      for (int k = 0; k < VN; ++k) {
+        float f = Elt<T>::to_f(xv[u].e[k]);
+        if (r) {
+          hv[u].e[k] = Elt<R>::from_f(f + Elt<R>::to_f(hv[u].e[k]));
+          f = Elt<R>::to_f(hv[u].e[k]);
+        }
+        ss = fmaf(f, f, ss);
+      }
+      if (r && there) hv[u].store(h + row * cols + c * VN);
+    }
+  }
+  const float s = rsqrtf(row_reduce<TPR, false>(ss, red[0]) / (float)cols + eps);
+  if (!QUANT && t == 0 && rstd && there) rstd[row] = s;
+  if constexpr (!QUANT) {
+#pragma unroll
+    for (int u = 0; u < CPT; ++u) {
+      const int c = t + u * TPR;
+      if (c < chunks) {
+#pragma unroll
+        for (int k = 0; k < VN; ++k)
+          xv[u].e[k] = Elt<T>::from_f(Elt<R>::to_f(hv[u].e[k]) * s * wv[u][k]);
+        if (there) xv[u].store(y + row * cols + c * VN);
+      }
+    }
+  } else {
+    float m = 0.f;
+#pragma unroll
+    for (int u = 0; u < CPT; ++u) {
+      const int c = t + u * TPR;
+      float mu = 0.f;
+#pragma unroll
+      for (int k = 0; k < VN; ++k) {
+        const float f = r ? Elt<R>::to_f(hv[u].e[k]) : Elt<T>::to_f(xv[u].e[k]);
+        wv[u][k] = f * s * wv[u][k];
+        if (c < chunks) mu = fmaxf(mu, fabsf(wv[u][k]));
+      }
+      if constexpr (BLOCK) {
+        // The 128 / VN chunks of a group lie in neighbouring lanes (a row of 8 lanes is
+        // shorter than a group).
+        constexpr int kLanes = 128 / VN < TPR ? 128 / VN : TPR;
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) mu = fmaxf(mu, __shfl_xor_sync(0xffffffffu, mu, o));
+        const float scale = fmaxf(mu / kE4m3Max, kMinScale), inv = 1.0f / scale;
+        if (c < chunks) {
+          if (t % kLanes == 0 && there)
+            scales[row * ((cols + 127) / 128) + c * VN / 128] = scale;
+#pragma unroll
+          for (int k = 0; k < VN; ++k) wv[u][k] *= inv;
+        }
+      } else {
+        m = fmaxf(m, mu);
+      }
+    }
+    float inv = 1.f;
+    if constexpr (!BLOCK) {
+      const float scale = fmaxf(row_reduce<TPR, true>(m, red[1]) / kE4m3Max, kMinScale);
+      if (t == 0 && there) scales[row] = scale;
+      inv = 1.0f / scale;
+    }
+#pragma unroll
+    for (int u = 0; u < CPT; ++u) {
+      const int c = t + u * TPR;
+      if (c < chunks && there) {
+        uint32_t o[VN / 4];
+#pragma unroll
+        for (int k = 0; k < VN; k += 4) {
+          const uint32_t lo = __nv_cvt_float2_to_fp8x2(
+              make_float2(wv[u][k] * inv, wv[u][k + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+          const uint32_t hi = __nv_cvt_float2_to_fp8x2(
+              make_float2(wv[u][k + 2] * inv, wv[u][k + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+          o[k / 4] = lo | hi << 16;
+        }
+        uint8_t* at = q + row * cols + c * VN;
+        if constexpr (VN == 8) __stcs(reinterpret_cast<uint2*>(at), make_uint2(o[0], o[1]));
+        else __stcs(reinterpret_cast<uint32_t*>(at), o[0]);
+      }
+    }
+  }
+}
+
+struct FwdArgs {
+  const void *x, *r, *w;
+  void *y, *q, *h;
+  float *scales, *rstd;
+  int64_t xs, rs, rows, cols;
+  int wd;
+  float eps;
+};
+
+template <typename T, typename R, bool QUANT, bool BLOCK, int TPR, int CPT>
+int launch_rows(const FwdArgs& a, cudaStream_t st) {
+  const int64_t grid = (a.rows + fwd_groups(TPR) - 1) / fwd_groups(TPR);
+  add_rmsnorm_rows<T, R, TPR, CPT, QUANT, BLOCK><<<(unsigned)grid, TPR <= 32 ? 256 : TPR, 0, st>>>(
+      static_cast<const T*>(a.x), a.xs, static_cast<const R*>(a.r), a.rs, a.w, a.wd,
+      static_cast<T*>(a.y), static_cast<uint8_t*>(a.q), a.scales, static_cast<R*>(a.h), a.rstd,
+      a.rows, (int)a.cols, a.eps);
+  return launch_status(QUANT ? "fk_add_rmsnorm_quant" : "fk_add_rmsnorm_fwd");
+}
+
+// Whether every row of x, r and the outputs is whole 16-byte chunks.
+template <typename T, typename R>
+bool rows_of_chunks(const FwdArgs& a) {
+  constexpr int VN = 16 / (int)sizeof(T);
+  return a.cols % VN == 0 && aligned16(a.x) && a.xs % VN == 0 && aligned16(a.w) &&
+         (!a.r || (aligned16(a.r) && a.rs * (int64_t)sizeof(R) % 16 == 0 && aligned16(a.h))) &&
+         (!a.y || aligned16(a.y)) && (!a.q || aligned16(a.q)) &&
+         a.rows < ((int64_t)1 << 31);
+}
+
+// Runs the chunk kernel where the rows allow it (at most 2048 chunks); -1 where they do not.
+template <typename T, typename R, bool QUANT, bool BLOCK>
+int rows_chunked(const FwdArgs& a, cudaStream_t st) {
+  if (!rows_of_chunks<T, R>(a)) return -1;
+  const int64_t chunks = a.cols / (16 / (int)sizeof(T));
+  if (chunks <= 8) return launch_rows<T, R, QUANT, BLOCK, 8, 1>(a, st);
+  if (chunks <= 32) return launch_rows<T, R, QUANT, BLOCK, 32, 1>(a, st);
+  if (chunks <= 128) return launch_rows<T, R, QUANT, BLOCK, 32, 4>(a, st);
+  if (chunks <= 256) return launch_rows<T, R, QUANT, BLOCK, 128, 2>(a, st);
+  if (chunks <= 512) return launch_rows<T, R, QUANT, BLOCK, 256, 2>(a, st);
+  if (chunks <= 1024) return launch_rows<T, R, QUANT, BLOCK, 512, 2>(a, st);
+  if (chunks <= 2048) return launch_rows<T, R, QUANT, BLOCK, 512, 4>(a, st);
+  return -1;
+}
+
 // ------------------------------------------------------------------ any shape -----------
 // One CTA per row, element loops.  h is re-read by the thread that wrote it.
 template <typename T, typename R>
@@ -173,6 +409,9 @@ inline size_t bwd_ws_bytes(int64_t rows, int64_t cols) {
 template <typename T, typename R>
 int fwd_t(const void* x, int64_t xs, const void* r, int64_t rs, const void* w, int wd, void* y,
           void* h, float* rstd, int64_t rows, int64_t cols, float eps, cudaStream_t st) {
+  const FwdArgs a{x, r, w, y, nullptr, h, nullptr, rstd, xs, rs, rows, cols, wd, eps};
+  const int done = rows_chunked<T, R, false, false>(a, st);
+  if (done >= 0) return done;
   add_rmsnorm_fwd_generic<T, R><<<row_grid(rows), 256, 0, st>>>(
       static_cast<const T*>(x), xs, static_cast<const R*>(r), rs, w, wd, static_cast<T*>(y),
       static_cast<R*>(h), rstd, rows, cols, eps);
@@ -194,6 +433,10 @@ template <typename T, typename R>
 int quant_t(const void* x, int64_t xs, const void* r, int64_t rs, const void* w, int wd, void* q,
             float* scales, void* h, int64_t rows, int64_t cols, int64_t block, float eps,
             cudaStream_t st) {
+  const FwdArgs a{x, r, w, nullptr, q, h, scales, nullptr, xs, rs, rows, cols, wd, eps};
+  const int done = block == cols ? rows_chunked<T, R, true, false>(a, st)
+                                 : rows_chunked<T, R, true, true>(a, st);
+  if (done >= 0) return done;
   add_rmsnorm_quant_generic<T, R><<<row_grid(rows), 256, 0, st>>>(
       static_cast<const T*>(x), xs, static_cast<const R*>(r), rs, w, wd,
       static_cast<uint8_t*>(q), scales, static_cast<R*>(h), rows, cols, block, eps);
