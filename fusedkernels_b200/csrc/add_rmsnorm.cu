@@ -10,12 +10,14 @@
 // reads, so forward and backward see the same row.  T is the type of x and y, R the type
 // of the residual stream (T or fp32); every statistic is fp32.
 #include "common.cuh"
+#include "ptx.cuh"
 
 #include <cuda_fp8.h>
 
 namespace fk {
 namespace {
 
+constexpr int kMaxGridPerSm = 8;  // CTAs of a backward grid, and partial rows of dw, per SM
 constexpr float kE4m3Max = 448.f;
 constexpr float kMinScale = 1.17549435e-38f;  // 2^-126: a row of zeros keeps a usable scale
 
@@ -282,6 +284,289 @@ int rows_chunked(const FwdArgs& a, cudaStream_t st) {
   return -1;
 }
 
+// ------------------------------------------------------------------ backward, chunks ----
+// Persistent CTAs, so that dw is summed in registers: a thread has the same columns in every
+// row it meets.  Each CTA leaves one partial row of dw; a second kernel adds those up.
+struct BwdArgs {
+  const void *dy, *dh, *h, *w;
+  const float* rstd;
+  void *dx, *dr;
+  float* part;
+  int64_t dys, dhs;
+  int rows, cols, wd;
+};
+
+// g of one chunk from its dy, h, dh; stores dx (and dr).
+template <typename T, typename R, int VN>
+__device__ __forceinline__ void bwd_store(const Chunk<T, VN>& dy, const Chunk<R, VN>& h,
+                                          const Chunk<R, VN>& dh, const float (&w)[VN], float s,
+                                          float c2, bool has_dh, T* dx, R* dr) {
+  Chunk<T, VN> ox;
+  Chunk<R, VN> orr;
+#pragma unroll
+  for (int k = 0; k < VN; ++k) {
+    float g = s * (w[k] * Elt<T>::to_f(dy.e[k])) - Elt<R>::to_f(h.e[k]) * c2;
+    if (has_dh) g += Elt<R>::to_f(dh.e[k]);
+    ox.e[k] = Elt<T>::from_f(g);
+    orr.e[k] = Elt<R>::from_f(g);
+  }
+  ox.store(dx);
+  if (sizeof(T) != sizeof(R)) orr.store(dr);
+}
+
+// Rows of at most 128 chunks: TPR lanes of a warp take a row (no CTA barrier per row), and the
+// next row is loaded while this one is worked on.
+template <typename T, typename R, int TPR, int CPT>
+__global__ void __launch_bounds__(256) add_rmsnorm_bwd_lanes(BwdArgs a) {
+  constexpr int VN = 16 / (int)sizeof(T), kGroups = 256 / TPR;
+  extern __shared__ float sum[];  // [cols]
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const int chunks = a.cols / VN;
+  const T* dy = static_cast<const T*>(a.dy);
+  const R *dh = static_cast<const R*>(a.dh), *h = static_cast<const R*>(a.h);
+  const float inv_cols = 1.0f / (float)a.cols;
+  float wv[CPT][VN], acc[CPT][VN];
+#pragma unroll
+  for (int u = 0; u < CPT; ++u) {
+    const int c = t + u * TPR;
+#pragma unroll
+    for (int k = 0; k < VN; ++k) wv[u][k] = acc[u][k] = 0.f;
+    if (c < chunks) load_weights<VN>(a.w, a.wd, c * VN, wv[u]);
+  }
+  Chunk<T, VN> ndy[CPT];
+  Chunk<R, VN> nh[CPT], ndh[CPT];
+  float ns = 0.f;
+  auto load = [&](int row) {
+    if (row >= a.rows) return;
+    ns = __ldg(a.rstd + row);
+#pragma unroll
+    for (int u = 0; u < CPT; ++u) {
+      const int c = t + u * TPR;
+      if (c < chunks) {
+        ndy[u].load(dy + row * a.dys + c * VN);
+        nh[u].load(h + (int64_t)row * a.cols + c * VN);
+        if (dh) ndh[u].load(dh + row * a.dhs + c * VN);
+      }
+    }
+  };
+  const int step = gridDim.x * kGroups;
+  // Whole warps go round together: a group past the last row only joins the shuffles.
+  const int first = blockIdx.x * kGroups + group, warp_first = first - (threadIdx.x & 31) / TPR;
+  load(first);
+  for (int row = first, wr = warp_first; wr < a.rows; row += step, wr += step) {
+    const bool there = row < a.rows;
+    Chunk<T, VN> vdy[CPT];
+    Chunk<R, VN> vh[CPT], vdh[CPT];
+    const float s = ns;
+#pragma unroll
+    for (int u = 0; u < CPT; ++u) {
+      vdy[u] = ndy[u];
+      vh[u] = nh[u];
+      vdh[u] = ndh[u];
+    }
+    load(row + step);
+    float dot = 0.f;
+#pragma unroll
+    for (int u = 0; u < CPT; ++u)
+      if (there && t + u * TPR < chunks)
+#pragma unroll
+        for (int k = 0; k < VN; ++k) {
+          const float d = Elt<T>::to_f(vdy[u].e[k]), hv = Elt<R>::to_f(vh[u].e[k]);
+          dot = fmaf(wv[u][k] * d, hv, dot);
+          acc[u][k] = fmaf(d * hv, s, acc[u][k]);
+        }
+    dot = row_reduce<TPR, false>(dot, nullptr);
+    const float c2 = s * s * s * (dot * inv_cols);
+#pragma unroll
+    for (int u = 0; u < CPT; ++u) {
+      const int c = t + u * TPR;
+      if (there && c < chunks)
+        bwd_store<T, R, VN>(vdy[u], vh[u], vdh[u], wv[u], s, c2, dh != nullptr,
+                            static_cast<T*>(a.dx) + (int64_t)row * a.cols + c * VN,
+                            static_cast<R*>(a.dr) + (int64_t)row * a.cols + c * VN);
+    }
+  }
+  for (int c = threadIdx.x; c < a.cols; c += 256) sum[c] = 0.f;
+  for (int g = 0; g < kGroups; ++g) {  // the groups' sums, in their order
+    __syncthreads();
+    if (group == g)
+#pragma unroll
+      for (int u = 0; u < CPT; ++u) {
+        const int c = t + u * TPR;
+        if (c < chunks)
+#pragma unroll
+          for (int k = 0; k < VN; ++k) sum[c * VN + k] += acc[u][k];
+      }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.cols; c += 256)
+    a.part[(int64_t)blockIdx.x * a.cols + c] = sum[c];
+}
+
+// Longer rows: the CTA takes a row.  Rows of dy, h and dh arrive in a ring of shared-memory
+// stages by cp.async.bulk; a stage is refilled as soon as all threads have its chunks in
+// registers, which the reduction's barrier tells.
+constexpr int kBwdMaxStages = 4;
+template <typename T, typename R, int THREADS, int CPT>
+__global__ void __launch_bounds__(THREADS) add_rmsnorm_bwd_ring(BwdArgs a, int stages) {
+  constexpr int VN = 16 / (int)sizeof(T);
+  using CT = Chunk<T, VN>;
+  using CR = Chunk<R, VN>;
+  extern __shared__ __align__(128) unsigned char ring[];
+  __shared__ __align__(8) uint64_t full[kBwdMaxStages];
+  __shared__ float red[2][32];
+  const int tid = threadIdx.x, chunks = a.cols / VN;
+  const T* dy = static_cast<const T*>(a.dy);
+  const R *dh = static_cast<const R*>(a.dh), *h = static_cast<const R*>(a.h);
+  const uint32_t tb = (uint32_t)a.cols * sizeof(T), rb = (uint32_t)a.cols * sizeof(R);
+  const uint32_t stage_bytes = tb + (dh ? 2 : 1) * rb;
+  const float inv_cols = 1.0f / (float)a.cols;
+  float wv[CPT][VN], acc[CPT][VN];
+#pragma unroll
+  for (int u = 0; u < CPT; ++u) {
+    const int c = tid + u * THREADS;
+#pragma unroll
+    for (int k = 0; k < VN; ++k) wv[u][k] = acc[u][k] = 0.f;
+    if (c < chunks) load_weights<VN>(a.w, a.wd, c * VN, wv[u]);
+  }
+  auto issue = [&](int row, int q) {
+    if (row >= a.rows) return;
+    unsigned char* at = ring + q * stage_bytes;
+    ptx::fence_proxy_async_smem();
+    ptx::mbar_arrive_expect_tx(&full[q], stage_bytes);
+    ptx::bulk_g2s(at, dy + row * a.dys, tb, &full[q]);
+    ptx::bulk_g2s(at + tb, h + (int64_t)row * a.cols, rb, &full[q]);
+    if (dh) ptx::bulk_g2s(at + tb + rb, dh + row * a.dhs, rb, &full[q]);
+  };
+  const int step = gridDim.x;
+  if (tid == 0) {
+    for (int q = 0; q < stages; ++q) ptx::mbar_init(&full[q], 1);
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async_smem();
+    for (int q = 0; q < stages; ++q) issue(blockIdx.x + q * step, q);
+  }
+  __syncthreads();
+  bool ok = true;
+  int q = 0, phase = 0, parity = 0;
+  float ns = (int)blockIdx.x < a.rows ? __ldg(a.rstd + blockIdx.x) : 0.f;
+  for (int row = blockIdx.x; row < a.rows; row += step) {
+    const float s = ns;
+    if (row + step < a.rows) ns = __ldg(a.rstd + row + step);
+    ok = ptx::mbar_wait(&full[q], (uint32_t)phase, ok ? (1u << 26) : 1u) && ok;
+    const unsigned char* at = ring + q * stage_bytes;
+    CT vdy[CPT];
+    CR vh[CPT], vdh[CPT];
+    float dot = 0.f;
+#pragma unroll
+    for (int u = 0; u < CPT; ++u) {
+      const int c = tid + u * THREADS;
+      if (c < chunks) {
+        vdy[u].u[0] = reinterpret_cast<const uint4*>(at)[c];
+#pragma unroll
+        for (int i = 0; i < CR::N16; ++i) {
+          vh[u].u[i] = reinterpret_cast<const uint4*>(at + tb)[c * CR::N16 + i];
+          if (dh) vdh[u].u[i] = reinterpret_cast<const uint4*>(at + tb + rb)[c * CR::N16 + i];
+        }
+#pragma unroll
+        for (int k = 0; k < VN; ++k) {
+          const float d = Elt<T>::to_f(vdy[u].e[k]), hv = Elt<R>::to_f(vh[u].e[k]);
+          dot = fmaf(wv[u][k] * d, hv, dot);
+          acc[u][k] = fmaf(d * hv, s, acc[u][k]);
+        }
+      }
+    }
+    dot = row_reduce<THREADS, false>(dot, red[parity]);  // its barrier frees the stage
+    if (tid == 0) issue(row + stages * step, q);
+    // (A wait that ran out poisons the row.)
+    const float c2 = ok ? s * s * s * (dot * inv_cols) : __int_as_float(0x7fc00000);
+#pragma unroll
+    for (int u = 0; u < CPT; ++u) {
+      const int c = tid + u * THREADS;
+      if (c < chunks)
+        bwd_store<T, R, VN>(vdy[u], vh[u], vdh[u], wv[u], s, c2, dh != nullptr,
+                            static_cast<T*>(a.dx) + (int64_t)row * a.cols + c * VN,
+                            static_cast<R*>(a.dr) + (int64_t)row * a.cols + c * VN);
+    }
+    parity ^= 1;
+    if (++q == stages) {
+      q = 0;
+      phase ^= 1;
+    }
+  }
+  float* prow = a.part + (int64_t)blockIdx.x * a.cols;
+#pragma unroll
+  for (int u = 0; u < CPT; ++u) {
+    const int c = tid + u * THREADS;
+    if (c < chunks)
+#pragma unroll
+      for (int k = 0; k < VN; k += 4)
+        *reinterpret_cast<float4*>(prow + c * VN + k) =
+            make_float4(acc[u][k], acc[u][k + 1], acc[u][k + 2], acc[u][k + 3]);
+  }
+}
+
+// CTAs of KERNEL that an SM holds, looked up again when the device or the sizes change.
+template <auto KERNEL>
+int resident_ctas(int threads, int smem) {
+  static thread_local int asked_dev = -1, asked_smem, answer;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+  if (asked_dev != dev || asked_smem != smem) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&answer, KERNEL, threads, (size_t)smem) !=
+            cudaSuccess ||
+        answer < 1) {
+      cudaGetLastError();
+      answer = 1;
+    }
+    asked_dev = dev;
+    asked_smem = smem;
+  }
+  return answer < kMaxGridPerSm ? answer : kMaxGridPerSm;
+}
+
+template <typename T, typename R, int TPR, int CPT>
+int launch_bwd_lanes(const BwdArgs& a, int* grid, cudaStream_t st) {
+  constexpr auto kern = add_rmsnorm_bwd_lanes<T, R, TPR, CPT>;
+  const int smem = a.cols * 4, groups = 256 / TPR;
+  const int most = num_sms() * resident_ctas<kern>(256, smem);
+  const int want = (a.rows + groups - 1) / groups;
+  *grid = want < most ? want : most;
+  kern<<<*grid, 256, smem, st>>>(a);
+  return launch_status("fk_add_rmsnorm_bwd");
+}
+
+template <typename T, typename R, int THREADS, int CPT>
+int launch_bwd_ring(const BwdArgs& a, int* grid, cudaStream_t st) {
+  constexpr auto kern = add_rmsnorm_bwd_ring<T, R, THREADS, CPT>;
+  allow_shared_memory<kern>(1024);
+  const int stage = a.cols * ((int)sizeof(T) + (a.dh ? 2 : 1) * (int)sizeof(R));
+  int stages = 72 * 1024 / stage;
+  stages = stages < 2 ? 2 : stages > 3 ? 3 : stages;
+  const int smem = stages * stage;
+  const int most = num_sms() * resident_ctas<kern>(THREADS, smem);
+  *grid = a.rows < most ? a.rows : most;
+  kern<<<*grid, THREADS, smem, st>>>(a, stages);
+  return launch_status("fk_add_rmsnorm_bwd");
+}
+
+// Runs a chunk kernel where the rows allow it; -1 where they do not.
+template <typename T, typename R>
+int bwd_chunked(const BwdArgs& a, int* grid, cudaStream_t st) {
+  constexpr int VN = 16 / (int)sizeof(T);
+  const bool fits = a.cols % VN == 0 && aligned16(a.dy) && a.dys % VN == 0 && aligned16(a.h) &&
+                    (!a.dh || (aligned16(a.dh) && a.dhs * (int64_t)sizeof(R) % 16 == 0)) &&
+                    aligned16(a.w) && aligned16(a.dx) && aligned16(a.dr);
+  if (!fits) return -1;
+  const int chunks = a.cols / VN;
+  if (chunks <= 8) return launch_bwd_lanes<T, R, 8, 1>(a, grid, st);
+  if (chunks <= 32) return launch_bwd_lanes<T, R, 32, 1>(a, grid, st);
+  if (chunks <= 64) return launch_bwd_lanes<T, R, 32, 2>(a, grid, st);
+  if (chunks <= 256) return launch_bwd_ring<T, R, 128, 2>(a, grid, st);
+  if (chunks <= 512) return launch_bwd_ring<T, R, 256, 2>(a, grid, st);
+  if (chunks <= 1024) return launch_bwd_ring<T, R, 512, 2>(a, grid, st);
+  return -1;
+}
+
 // ------------------------------------------------------------------ any shape -----------
 // One CTA per row, element loops.  h is re-read by the thread that wrote it.
 template <typename T, typename R>
@@ -397,7 +682,6 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_dw_reduce(const float* __res
   }
 }
 
-constexpr int kMaxGridPerSm = 8;
 inline int row_grid(int64_t rows) {
   const int64_t g = (int64_t)num_sms() * kMaxGridPerSm;
   return (int)(rows < g ? rows : g);
@@ -422,6 +706,12 @@ template <typename T, typename R>
 int bwd_t(const void* dy, int64_t dys, const void* dh, int64_t dhs, const void* h, const void* w,
           int wd, const float* rstd, void* dx, void* dr, float* part, int64_t rows, int64_t cols,
           int* grid, cudaStream_t st) {
+  if (rows < ((int64_t)1 << 31) - (1 << 20) && cols < (1 << 20)) {
+    const BwdArgs a{dy,  dh,  h,         w,         rstd, dx, dr,
+                    part, dys, dhs, (int)rows, (int)cols, wd};
+    const int done = bwd_chunked<T, R>(a, grid, st);
+    if (done >= 0) return done;
+  }
   *grid = row_grid(rows);
   add_rmsnorm_bwd_generic<T, R><<<*grid, 256, 0, st>>>(
       static_cast<const T*>(dy), dys, static_cast<const R*>(dh), dhs, static_cast<const R*>(h), w,
