@@ -48,6 +48,11 @@ __device__ __forceinline__ float block_max(float v, float* red) {
   return m;
 }
 
+// Scale of a group with largest magnitude m (1 / 448 rounded: 1 ulp).
+__device__ __forceinline__ float scale_of(float m) {
+  return fmaxf(m * (1.0f / kE4m3Max), kMinScale);
+}
+
 // ------------------------------------------------------------------ 16-byte chunks ------
 // A chunk is 16 bytes of x (VN elements) and the same elements of the residual: one 16-byte
 // load, or two where the residual is fp32 beside 16-bit x.
@@ -202,7 +207,7 @@ __global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR) add_rmsnorm_rows(
         constexpr int kLanes = 128 / VN < TPR ? 128 / VN : TPR;
 #pragma unroll
         for (int o = kLanes / 2; o > 0; o >>= 1) mu = fmaxf(mu, __shfl_xor_sync(0xffffffffu, mu, o));
-        const float scale = fmaxf(mu / kE4m3Max, kMinScale), inv = 1.0f / scale;
+        const float scale = scale_of(mu), inv = __fdividef(1.0f, scale);
         if (c < chunks) {
           if (t % kLanes == 0 && there)
             scales[row * ((cols + 127) / 128) + c * VN / 128] = scale;
@@ -215,9 +220,9 @@ __global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR) add_rmsnorm_rows(
     }
     float inv = 1.f;
     if constexpr (!BLOCK) {
-      const float scale = fmaxf(row_reduce<TPR, true>(m, red[1]) / kE4m3Max, kMinScale);
+      const float scale = scale_of(row_reduce<TPR, true>(m, red[1]));
       if (t == 0 && there) scales[row] = scale;
-      inv = 1.0f / scale;
+      inv = __fdividef(1.0f, scale);
     }
 #pragma unroll
     for (int u = 0; u < CPT; ++u) {
@@ -651,7 +656,7 @@ __global__ void __launch_bounds__(256) add_rmsnorm_quant_generic(
       const int64_t c0 = g * block, c1 = c0 + block < cols ? c0 + block : cols;
       float m = 0.f;
       for (int64_t c = c0 + threadIdx.x; c < c1; c += blockDim.x) m = fmaxf(m, fabsf(value(c)));
-      const float scale = fmaxf(block_max(m, red) / kE4m3Max, kMinScale);
+      const float scale = scale_of(block_max(m, red));
       if (threadIdx.x == 0) scales[row * groups + g] = scale;
       for (int64_t c = c0 + threadIdx.x; c < c1; c += blockDim.x)
         q[row * cols + c] = to_e4m3(value(c) / scale);
