@@ -13,6 +13,7 @@
 // for the two sums and once for its gradient, and the gradient at the listed ids is computed
 // from the logit itself, in 32 bits, and rounded once.
 #include "common.cuh"
+#include "exp.cuh"
 #include "ptx.cuh"
 
 namespace fk {
@@ -394,38 +395,13 @@ __global__ void __launch_bounds__(kGenericThreads) distill_rows_generic(
 // offset) are taken singly by the first CTA.  Logits and gradient have to have the same
 // offset from a 16-byte boundary in every row; other layouts take the generic kernel.
 constexpr int kMaxStages = 3;
-constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // exp(d) of a scaled difference d <= 0: 16-bit gradients round to 8 or 11 bits, so one ex2 is
 // exact enough; 32-bit ones take expf.
 template <typename T>
 __device__ __forceinline__ float exp_of(float d) { return ex2f(d * kLog2e); }
 template <>
 __device__ __forceinline__ float exp_of<float>(float d) { return expf(d); }
-
-// exp in 32 bits: 2^(d log2 e) with the product in two parts,
-// hi + lo (log2 e = kLog2e + kLog2eLow, the roundings of the products caught by FMAs), so that
-// the error stays that of ex2 (2 ulp) for any d: 2^hi * (1 + lo ln 2), lo being below 2^-16.
-// d is held at -200 from below (2^hi is 0 there), so that -inf does not meet its own residual.
-constexpr float kLog2eLow = 1.9259629911266174e-8f;
-constexpr float kLn2 = 0.69314718055994531f;
-__device__ __forceinline__ float max_or_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float exp2_of(float d) {
-  d = max_or_nan(d, -200.f);
-  const float hi = d * kLog2e;
-  const float lo = fmaf(d, kLog2eLow, fmaf(d, kLog2e, -hi));
-  const float p = ex2f(hi);
-  return fmaf(p * kLn2, lo, p);
-}
 
 template <typename T> struct Pair;  // two neighbouring elements
 template <> struct Pair<__nv_bfloat16> {

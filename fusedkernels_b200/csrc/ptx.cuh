@@ -101,6 +101,11 @@ __device__ __forceinline__ float ld_dsmem_f32(uint32_t cluster_addr) {
   return v;
 }
 
+__device__ __forceinline__ int ld_dsmem_s32(uint32_t cluster_addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
 // Address of the same shared object in CTA `rank`, from a generic pointer to this CTA's.
 __device__ __forceinline__ uint32_t peer_smem(const void* p, uint32_t rank) {
   return mapa(smem_u32(p), rank);
