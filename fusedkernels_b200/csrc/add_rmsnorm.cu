@@ -53,6 +53,10 @@ __device__ __forceinline__ float scale_of(float m) {
   return fmaxf(m * (1.0f / kE4m3Max), kMinScale);
 }
 
+__device__ __forceinline__ uint8_t to_e4m3(float v) {
+  return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+}
+
 // ------------------------------------------------------------------ 16-byte chunks ------
 // A chunk is 16 bytes of x (VN elements) and the same elements of the residual: one 16-byte
 // load, or two where the residual is fp32 beside 16-bit x.
@@ -577,6 +581,244 @@ int bwd_chunked(const BwdArgs& a, int* grid, cudaStream_t st) {
   return -1;
 }
 
+// ------------------------------------------------------------------ tiles ---------------
+// Contiguous rows of a width that is not whole chunks: 16 / sizeof(T) rows together are a
+// multiple of 16 bytes in every tensor, whatever the width.  A tile of some such rows comes to
+// shared memory by cp.async.bulk, a warp takes a row of it (single elements, no bank
+// conflicts), results go over the inputs and leave by bulk stores: memory sees whole lines
+// only.  The last rows, fewer than a unit, are copied element by element.
+//
+// Copies a tile's elements (whole: a multiple of 16 bytes, by the bulk unit).
+template <typename E>
+__device__ __forceinline__ void tile_in(E* dst, const E* src, int elements, bool whole,
+                                        uint64_t* bar) {
+  if (whole) {
+    if (threadIdx.x == 0) ptx::bulk_g2s(dst, src, (uint32_t)(elements * sizeof(E)), bar);
+  } else {
+    for (int i = threadIdx.x; i < elements; i += blockDim.x) dst[i] = src[i];
+  }
+}
+template <typename E>
+__device__ __forceinline__ void tile_out(E* dst, const E* src, int elements, bool whole) {
+  if (whole) {
+    if (threadIdx.x == 0) ptx::bulk_s2g(dst, src, (uint32_t)(elements * sizeof(E)));
+  } else {
+    for (int i = threadIdx.x; i < elements; i += blockDim.x) dst[i] = src[i];
+  }
+}
+inline __host__ __device__ int align128(int n) { return (n + 127) / 128 * 128; }
+
+constexpr int kTileThreads = 256;
+
+// Forward (QUANT: the 8-bit form; q leaves as single bytes, 32 of a warp side by side).
+template <typename T, typename R, bool QUANT>
+__global__ void __launch_bounds__(kTileThreads) add_rmsnorm_tile(FwdArgs a, int tile_rows,
+                                                                 int block) {
+  constexpr int kUnit = 16 / (int)sizeof(T);
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) uint64_t full;
+  const int cols = (int)a.cols, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row0 = (int64_t)blockIdx.x * tile_rows;
+  const int n = (int)(a.rows - row0 < tile_rows ? a.rows - row0 : tile_rows);
+  const bool whole = n % kUnit == 0;
+  T* xt = reinterpret_cast<T*>(smem);
+  R* ht = reinterpret_cast<R*>(smem + align128(tile_rows * cols * (int)sizeof(T)));
+  if (threadIdx.x == 0) {
+    ptx::mbar_init(&full, 1);
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async_smem();
+    if (whole) ptx::mbar_arrive_expect_tx(&full, (uint32_t)(n * cols * (sizeof(T) + (a.r ? sizeof(R) : 0))));
+  }
+  tile_in(xt, static_cast<const T*>(a.x) + row0 * cols, n * cols, whole, &full);
+  if (a.r) tile_in(ht, static_cast<const R*>(a.r) + row0 * cols, n * cols, whole, &full);
+  __syncthreads();
+  // (A wait that runs out poisons the tile.)
+  const bool ok = !whole || ptx::mbar_wait(&full, 0);
+  for (int i = warp; i < n; i += kTileThreads / 32) {
+    T* x = xt + i * cols;
+    R* h = ht + i * cols;
+    float ss = 0.f;
+#pragma unroll 4
+    for (int c = lane; c < cols; c += 32) {
+      float f = Elt<T>::to_f(x[c]);
+      if (a.r) {
+        const R hv = Elt<R>::from_f(f + Elt<R>::to_f(h[c]));
+        h[c] = hv;
+        f = Elt<R>::to_f(hv);
+      }
+      ss = fmaf(f, f, ss);
+    }
+    float s = rsqrtf(warp_sum(ss) / (float)cols + a.eps);
+    if (!ok) s = __int_as_float(0x7fc00000);
+    if constexpr (!QUANT) {
+      if (lane == 0 && a.rstd) a.rstd[row0 + i] = s;
+#pragma unroll 4
+      for (int c = lane; c < cols; c += 32)
+        x[c] = Elt<T>::from_f(Elt<R>::to_f(h[c]) * s * load_wd(a.w, a.wd, c));
+    } else {
+      auto y = [&](int c) {
+        return (a.r ? Elt<R>::to_f(h[c]) : Elt<T>::to_f(x[c])) * s * load_wd(a.w, a.wd, c);
+      };
+      uint8_t* q = static_cast<uint8_t*>(a.q) + (row0 + i) * cols;
+      const int groups = (cols + block - 1) / block;
+      for (int g = 0; g < groups; ++g) {
+        const int c0 = g * block, c1 = c0 + block < cols ? c0 + block : cols;
+        float m = 0.f;
+        for (int c = c0 + lane; c < c1; c += 32) m = fmaxf(m, fabsf(y(c)));
+        const float scale = scale_of(warp_max(m)), inv = __fdividef(1.0f, scale);
+        if (lane == 0) a.scales[(row0 + i) * groups + g] = scale;
+        for (int c = c0 + lane; c < c1; c += 32) q[c] = to_e4m3(y(c) * inv);
+      }
+    }
+  }
+  ptx::fence_proxy_async_smem();
+  __syncthreads();
+  if (!QUANT) tile_out(static_cast<T*>(a.y) + row0 * cols, xt, n * cols, whole);
+  if (a.r) tile_out(static_cast<R*>(a.h) + row0 * cols, ht, n * cols, whole);
+  if (threadIdx.x == 0) {
+    ptx::bulk_commit();
+    ptx::bulk_wait_read();
+  }
+}
+
+// Backward: persistent CTAs over the tiles.  Warps form the rows' dots, then threads go down
+// the tile's columns: gradient over dy and h, and the column's part of dw, which is kept in
+// shared memory for the CTA's tiles.
+template <typename T, typename R>
+__global__ void __launch_bounds__(kTileThreads) add_rmsnorm_bwd_tile(BwdArgs a, int tile_rows) {
+  constexpr int kUnit = 16 / (int)sizeof(T);
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) uint64_t full;
+  const int cols = a.cols, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tb = align128(tile_rows * cols * (int)sizeof(T));
+  const int rb = align128(tile_rows * cols * (int)sizeof(R));
+  T* dyt = reinterpret_cast<T*>(smem);
+  R* ht = reinterpret_cast<R*>(smem + tb);
+  R* dht = reinterpret_cast<R*>(smem + tb + rb);
+  float* acc = reinterpret_cast<float*>(smem + tb + (a.dh ? 2 : 1) * rb);  // [cols]
+  float2* coef = reinterpret_cast<float2*>(acc + (cols + 1) / 2 * 2);      // [tile_rows] (s, c2)
+  for (int c = threadIdx.x; c < cols; c += kTileThreads) acc[c] = 0.f;
+  if (threadIdx.x == 0) {
+    ptx::mbar_init(&full, 1);
+    ptx::fence_mbar_init();
+  }
+  __syncthreads();
+  const float inv_cols = 1.0f / (float)cols;
+  bool ok = true;
+  int phase = 0;
+  for (int row0 = blockIdx.x * tile_rows; row0 < a.rows; row0 += gridDim.x * tile_rows) {
+    const int n = a.rows - row0 < tile_rows ? a.rows - row0 : tile_rows, count = n * cols;
+    const bool whole = n % kUnit == 0;
+    const int64_t at = (int64_t)row0 * cols;
+    if (threadIdx.x == 0 && whole) {
+      ptx::fence_proxy_async_smem();
+      ptx::mbar_arrive_expect_tx(&full, (uint32_t)(count * (sizeof(T) + (a.dh ? 2 : 1) * sizeof(R))));
+    }
+    tile_in(dyt, static_cast<const T*>(a.dy) + at, count, whole, &full);
+    tile_in(ht, static_cast<const R*>(a.h) + at, count, whole, &full);
+    if (a.dh) tile_in(dht, static_cast<const R*>(a.dh) + at, count, whole, &full);
+    if (whole) {
+      ok = ptx::mbar_wait(&full, (uint32_t)phase, ok ? (1u << 26) : 1u) && ok;
+      phase ^= 1;
+    } else {
+      __syncthreads();
+    }
+    for (int i = warp; i < n; i += kTileThreads / 32) {
+      const T* dy = dyt + i * cols;
+      const R* h = ht + i * cols;
+      float dot = 0.f;
+#pragma unroll 4
+      for (int c = lane; c < cols; c += 32)
+        dot = fmaf(load_wd(a.w, a.wd, c) * Elt<T>::to_f(dy[c]), Elt<R>::to_f(h[c]), dot);
+      dot = warp_sum(dot);
+      if (lane == 0) {
+        const float s = a.rstd[row0 + i];
+        coef[i] = make_float2(s, ok ? s * s * s * (dot * inv_cols) : __int_as_float(0x7fc00000));
+      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < cols; c += kTileThreads) {
+      const float w = load_wd(a.w, a.wd, c);
+      float sum = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float2 k = coef[i];
+        const float d = Elt<T>::to_f(dyt[i * cols + c]), h = Elt<R>::to_f(ht[i * cols + c]);
+        float g = k.x * (w * d) - h * k.y;
+        if (a.dh) g += Elt<R>::to_f(dht[i * cols + c]);
+        sum = fmaf(d * h, k.x, sum);
+        dyt[i * cols + c] = Elt<T>::from_f(g);
+        if (sizeof(T) != sizeof(R)) ht[i * cols + c] = Elt<R>::from_f(g);
+      }
+      acc[c] += sum;  // a column is one thread's
+    }
+    ptx::fence_proxy_async_smem();
+    __syncthreads();
+    tile_out(static_cast<T*>(a.dx) + at, dyt, count, whole);
+    if (sizeof(T) != sizeof(R)) tile_out(static_cast<R*>(a.dr) + at, ht, count, whole);
+    if (threadIdx.x == 0) {
+      ptx::bulk_commit();
+      ptx::bulk_wait_read();
+    }
+    __syncthreads();  // the tile is free again
+  }
+  for (int c = threadIdx.x; c < cols; c += kTileThreads)
+    a.part[(int64_t)blockIdx.x * cols + c] = acc[c];
+}
+
+// Rows of a tile: units of 16 / sizeof(T) rows, about 32 KB of them, fewer where the rows are
+// too few for four tiles per SM; 0 where one unit does not fit `most` bytes.
+template <typename T>
+int tile_rows_for(int64_t rows, int64_t cols, int bytes_per_element, int most) {
+  constexpr int kUnit = 16 / (int)sizeof(T);
+  const int64_t unit = kUnit * cols * bytes_per_element;
+  if (unit + 1024 > most) return 0;
+  int64_t units = 32 * 1024 / unit;
+  const int64_t share = rows / ((int64_t)num_sms() * 4 * kUnit);
+  if (units > share) units = share;
+  if (units > 16) units = 16;
+  return kUnit * (int)(units < 1 ? 1 : units);
+}
+constexpr int kTileSmem = 222 * 1024;
+
+// Runs the tile kernel where the rows are contiguous and a unit of them fits; -1 elsewhere.
+template <typename T, typename R, bool QUANT>
+int fwd_tiled(const FwdArgs& a, int64_t block, cudaStream_t st) {
+  if (a.xs != a.cols || (a.r && a.rs != a.cols) || !aligned16(a.x) || !aligned16(a.r) ||
+      !aligned16(a.y) || !aligned16(a.h) || a.cols > 16384 || a.rows >= (int64_t)1 << 31)
+    return -1;
+  const int n = tile_rows_for<T>(a.rows, a.cols, (int)sizeof(T) + (a.r ? (int)sizeof(R) : 0),
+                                 kTileSmem);
+  if (n == 0) return -1;
+  constexpr auto kern = add_rmsnorm_tile<T, R, QUANT>;
+  allow_shared_memory<kern>(1024);
+  const int smem = align128(n * (int)a.cols * (int)sizeof(T)) +
+                   (a.r ? align128(n * (int)a.cols * (int)sizeof(R)) : 0);
+  const int64_t grid = (a.rows + n - 1) / n;
+  kern<<<(unsigned)grid, kTileThreads, smem, st>>>(a, n, (int)block);
+  return launch_status(QUANT ? "fk_add_rmsnorm_quant" : "fk_add_rmsnorm_fwd");
+}
+
+template <typename T, typename R>
+int bwd_tiled(const BwdArgs& a, int* grid, cudaStream_t st) {
+  const int per = (int)sizeof(T) + (a.dh ? 2 : 1) * (int)sizeof(R);
+  if (a.dys != a.cols || (a.dh && a.dhs != a.cols) || !aligned16(a.dy) || !aligned16(a.dh) ||
+      !aligned16(a.h) || !aligned16(a.dx) || !aligned16(a.dr) || a.cols > 16384)
+    return -1;
+  const int n = tile_rows_for<T>(a.rows, a.cols, per, kTileSmem - a.cols * 4);
+  if (n == 0) return -1;
+  constexpr auto kern = add_rmsnorm_bwd_tile<T, R>;
+  allow_shared_memory<kern>(1024);
+  const int smem = align128(n * a.cols * (int)sizeof(T)) +
+                   (a.dh ? 2 : 1) * align128(n * a.cols * (int)sizeof(R)) + (a.cols + 1) / 2 * 8 +
+                   n * 8;
+  const int64_t want = ((int64_t)a.rows + n - 1) / n;
+  const int most = num_sms() * resident_ctas<kern>(kTileThreads, smem);
+  *grid = (int)(want < most ? want : most);
+  kern<<<*grid, kTileThreads, smem, st>>>(a, n);
+  return launch_status("fk_add_rmsnorm_bwd");
+}
+
 // ------------------------------------------------------------------ any shape -----------
 // One CTA per row, element loops.  h is re-read by the thread that wrote it.
 template <typename T, typename R>
@@ -626,10 +868,6 @@ __global__ void __launch_bounds__(256) add_rmsnorm_bwd_generic(
       if (dr) dr[row * cols + c] = Elt<R>::from_f(g);
     }
   }
-}
-
-__device__ __forceinline__ uint8_t to_e4m3(float v) {
-  return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
 }
 
 // r == nullptr: h is x itself and is not written.
@@ -704,7 +942,8 @@ template <typename T, typename R>
 int fwd_t(const void* x, int64_t xs, const void* r, int64_t rs, const void* w, int wd, void* y,
           void* h, float* rstd, int64_t rows, int64_t cols, float eps, cudaStream_t st) {
   const FwdArgs a{x, r, w, y, nullptr, h, nullptr, rstd, xs, rs, rows, cols, wd, eps};
-  const int done = rows_chunked<T, R, false, false>(a, st);
+  int done = rows_chunked<T, R, false, false>(a, st);
+  if (done < 0) done = fwd_tiled<T, R, false>(a, 0, st);
   if (done >= 0) return done;
   add_rmsnorm_fwd_generic<T, R><<<row_grid(rows), 256, 0, st>>>(
       static_cast<const T*>(x), xs, static_cast<const R*>(r), rs, w, wd, static_cast<T*>(y),
@@ -719,7 +958,8 @@ int bwd_t(const void* dy, int64_t dys, const void* dh, int64_t dhs, const void* 
   if (rows < ((int64_t)1 << 31) - (1 << 20) && cols < (1 << 20)) {
     const BwdArgs a{dy,  dh,  h,         w,         rstd, dx, dr,
                     part, dys, dhs, (int)rows, (int)cols, wd};
-    const int done = bwd_chunked<T, R>(a, grid, st);
+    int done = bwd_chunked<T, R>(a, grid, st);
+    if (done < 0) done = bwd_tiled<T, R>(a, grid, st);
     if (done >= 0) return done;
   }
   *grid = row_grid(rows);
@@ -734,8 +974,9 @@ int quant_t(const void* x, int64_t xs, const void* r, int64_t rs, const void* w,
             float* scales, void* h, int64_t rows, int64_t cols, int64_t block, float eps,
             cudaStream_t st) {
   const FwdArgs a{x, r, w, nullptr, q, h, scales, nullptr, xs, rs, rows, cols, wd, eps};
-  const int done = block == cols ? rows_chunked<T, R, true, false>(a, st)
-                                 : rows_chunked<T, R, true, true>(a, st);
+  int done = block == cols ? rows_chunked<T, R, true, false>(a, st)
+                           : rows_chunked<T, R, true, true>(a, st);
+  if (done < 0) done = fwd_tiled<T, R, true>(a, block, st);
   if (done >= 0) return done;
   add_rmsnorm_quant_generic<T, R><<<row_grid(rows), 256, 0, st>>>(
       static_cast<const T*>(x), xs, static_cast<const R*>(r), rs, w, wd,

@@ -77,6 +77,18 @@ def test_many_rows(types):
     assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+@pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("shape", [(10007, 33), (20005, 130), (9, 2001), (17, 7001)], ids=str)
+def test_odd_widths(shape, types):
+    """Widths that are not whole 16-byte packets: many short rows, rows left over at the end,
+    rows too long to be gathered in shared memory."""
+    x, r, w, dy, dh = inputs(shape, *types, FP, seed=30 + shape[1])
+    check(x, r, w, dy, dh, *leaves(x, r, w))
+    check(x, r, w, dy, None, *leaves(x, r, w))
+    for block in (None, 128):
+        check_quant(x, r, w, block)
+
+
 def test_one_output_used():
     x, r, w, dy, dh = inputs((30, 256), BF, FP, FP, seed=5)
     check(x, r, w, dy, None, *leaves(x, r, w))
