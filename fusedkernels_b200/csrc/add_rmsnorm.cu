@@ -17,6 +17,7 @@
 namespace fk {
 namespace {
 
+constexpr uint32_t kPolls = 1u << 21;  // of a wait, before it gives up
 constexpr int kMaxGridPerSm = 8;  // CTAs of a backward grid, and partial rows of dw, per SM
 constexpr float kE4m3Max = 448.f;
 constexpr float kMinScale = 1.17549435e-38f;  // 2^-126: a row of zeros keeps a usable scale
@@ -466,7 +467,7 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_bwd_ring(BwdArgs a, int s
   for (int row = blockIdx.x; row < a.rows; row += step) {
     const float s = ns;
     if (row + step < a.rows) ns = __ldg(a.rstd + row + step);
-    ok = ptx::mbar_wait(&full[q], (uint32_t)phase, ok ? (1u << 26) : 1u) && ok;
+    ok = ptx::mbar_wait(&full[q], (uint32_t)phase, ok ? kPolls : 1u) && ok;
     const unsigned char* at = ring + q * stage_bytes;
     CT vdy[CPT];
     CR vh[CPT], vdh[CPT];
@@ -633,7 +634,7 @@ __global__ void __launch_bounds__(kTileThreads) add_rmsnorm_tile(FwdArgs a, int 
   if (a.r) tile_in(ht, static_cast<const R*>(a.r) + row0 * cols, n * cols, whole, &full);
   __syncthreads();
   // (A wait that runs out poisons the tile.)
-  const bool ok = !whole || ptx::mbar_wait(&full, 0);
+  const bool ok = !whole || ptx::mbar_wait(&full, 0, kPolls);
   for (int i = warp; i < n; i += kTileThreads / 32) {
     T* x = xt + i * cols;
     R* h = ht + i * cols;
@@ -718,7 +719,7 @@ __global__ void __launch_bounds__(kTileThreads) add_rmsnorm_bwd_tile(BwdArgs a, 
     tile_in(ht, static_cast<const R*>(a.h) + at, count, whole, &full);
     if (a.dh) tile_in(dht, static_cast<const R*>(a.dh) + at, count, whole, &full);
     if (whole) {
-      ok = ptx::mbar_wait(&full, (uint32_t)phase, ok ? (1u << 26) : 1u) && ok;
+      ok = ptx::mbar_wait(&full, (uint32_t)phase, ok ? kPolls : 1u) && ok;
       phase ^= 1;
     } else {
       __syncthreads();

@@ -126,8 +126,9 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) distill_teacher(
       }
     }
     m = group_max(m);
-    const bool held = m != -INFINITY || group_any(nan);
+    nan = group_any(nan);  // (votes are for the whole warp: never behind a row's condition)
     bad = group_any(bad);
+    const bool held = m != -INFINITY || nan;
     __syncwarp();
     float z = 0.f;
     unsigned open = 0;  // this lane's slots that are not settled
@@ -395,6 +396,7 @@ __global__ void __launch_bounds__(kGenericThreads) distill_rows_generic(
 // offset) are taken singly by the first CTA.  Logits and gradient have to have the same
 // offset from a 16-byte boundary in every row; other layouts take the generic kernel.
 constexpr int kMaxStages = 3;
+constexpr uint32_t kPolls = 1u << 21;  // of a wait, before it gives up
 
 // exp(d) of a scaled difference d <= 0: 16-bit gradients round to 8 or 11 bits, so one ex2 is
 // exact enough; 32-bit ones take expf.
@@ -567,18 +569,23 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
       else if (tid >= 32 && tid - 32 < a.n_cols - tail) xs_at = tail + tid - 32;
       if (xs_at >= 0) xs = Elt<T>::to_f(src[xs_at]);
     }
-    ok = ptx::mbar_wait(&full[q], (uint32_t)phase, ok ? (1u << 26) : 1u) && ok;
+    ok = ptx::mbar_wait(&full[q], (uint32_t)phase, ok ? kPolls : 1u) && ok;
     const unsigned char* stage = ring + q * stage_bytes;
     PK p[KP];
+    // All but the last packet of every thread are there as a rule (one branch for the row).
+    const bool most_full = M != kTwo && (KP - 1) * THREADS <= sl.count;
+    const uint4* at = reinterpret_cast<const uint4*>(stage) + tid;
+    constexpr uint32_t w = Pair<T>::kNegInf;
+    if (most_full) {
 #pragma unroll
-    for (int u = 0; u < KP; ++u) {
-      const uint4* at = reinterpret_cast<const uint4*>(stage) + tid + u * THREADS;
-      if ((u + 1) * THREADS <= sl.count) {
-        p[u].u = *at;
-      } else {
-        constexpr uint32_t w = Pair<T>::kNegInf;
+      for (int u = 0; u + 1 < KP; ++u) p[u].u = at[u * THREADS];
+      p[KP - 1].u = make_uint4(w, w, w, w);
+      if (tid + (KP - 1) * THREADS < sl.count) p[KP - 1].u = at[(KP - 1) * THREADS];
+    } else {
+#pragma unroll
+      for (int u = 0; u < KP; ++u) {
         p[u].u = make_uint4(w, w, w, w);
-        if (tid + u * THREADS < sl.count) p[u].u = *at;
+        if (tid + u * THREADS < sl.count) p[u].u = at[u * THREADS];
       }
     }
     // Listed elements of this slice: the same thread handles a listed place all through.
@@ -634,13 +641,20 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
       for (int k = 0; k < NP; ++k) {
         const float2 x = p[u].p[k].f();
         float2 f, f1 = make_float2(0.f, 0.f);
-        exp_one(x.x, f.x, f1.x);
-        exp_one(x.y, f.y, f1.y);
-        z.x += f.x;
-        z.y += f.y;
-        if constexpr (M != kOne) {
-          z1.x += f1.x;
-          z1.y += f1.y;
+        if constexpr (sizeof(T) == 2 && M != kTwo) {
+          const float2 t = __ffma2_rn(x, make_float2(ct_row, ct_row), make_float2(nb_t, nb_t));
+          f = make_float2(ex2f(t.x), ex2f(t.y));
+          z = __fadd2_rn(z, f);
+          if constexpr (M == kSquare) z1 = __ffma2_rn(f, f, z1);
+        } else {
+          exp_one(x.x, f.x, f1.x);
+          exp_one(x.y, f.y, f1.y);
+          z.x += f.x;
+          z.y += f.y;
+          if constexpr (M != kOne) {
+            z1.x += f1.x;
+            z1.y += f1.y;
+          }
         }
         if constexpr (KEEP) {
           e[u][k] = f;
@@ -662,7 +676,7 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
         __syncwarp();
       }
       read_ahead(row + step);
-      ok = ptx::mbar_wait(&xbar[xb], (uint32_t)xphase, ok ? (1u << 26) : 1u) && ok;
+      ok = ptx::mbar_wait(&xbar[xb], (uint32_t)xphase, ok ? kPolls : 1u) && ok;
       const float4 f = xch[xb][lane & (C - 1)];
       const bool copy = (lane & 7) >= C;  // of a smaller cluster: counted once
       st = join<T, M, 8>(Stat{f.x, copy ? 0.f : f.y, copy ? 0.f : f.z}, inv_t);
@@ -731,10 +745,15 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
               o.p[k].set(g);
             } else {
               const float2 x = p[u].p[k].f();
-              o.p[k].set(make_float2(dense(x.x), dense(x.y)));
+              if constexpr (sizeof(T) == 2 && M == kOne) {
+                const float2 t = __ffma2_rn(x, make_float2(ct_row, ct_row), make_float2(ot, ot));
+                o.p[k].set(make_float2(ex2f(t.x), ex2f(t.y)));
+              } else {
+                o.p[k].set(make_float2(dense(x.x), dense(x.y)));
+              }
             }
           }
-          if ((u + 1) * THREADS <= sl.count || tid + u * THREADS < sl.count)
+          if ((u + 1 < KP && most_full) || tid + u * THREADS < sl.count)
             __stcs(out + u * THREADS, o.u);
         }
         if (xs_at >= 0) dst[xs_at] = Elt<T>::from_f(dense(xs));
@@ -855,8 +874,9 @@ int rows_mode(const T* lp, int64_t ls, T* gp, int64_t gs, const RowArgs& a, cuda
   constexpr bool keep = sizeof(T) == 4 && M != kTwo;
   if (per <= 128) return launch_rows<T, M, true, 128, 1, 8>(lp, ls, gp, gs, lc, bytes, a, st);
   if (per <= 512) return launch_rows<T, M, keep, 128, 4, 8>(lp, ls, gp, gs, lc, bytes, a, st);
-  if (per <= 2048) return launch_rows<T, M, keep, 128, 16, 4>(lp, ls, gp, gs, lc, bytes, a, st);
-  return launch_rows<T, M, keep, 256, 16, 2>(lp, ls, gp, gs, lc, bytes, a, st);
+  constexpr int ctas = sizeof(T) == 2 && M == kTwo ? 3 : 4;
+  if (per <= 2048) return launch_rows<T, M, keep, 128, 16, ctas>(lp, ls, gp, gs, lc, bytes, a, st);
+  return launch_rows<T, M, keep, 256, 16, ctas / 2>(lp, ls, gp, gs, lc, bytes, a, st);
 }
 
 template <typename T>

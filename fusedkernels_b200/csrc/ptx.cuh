@@ -99,6 +99,7 @@ __device__ __forceinline__ uint32_t nclusters_x() {
 }
 // Full cluster barrier with release/acquire semantics (all threads of all CTAs).
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();  // the aligned forms want whole warps
   asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
                "barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

@@ -112,6 +112,32 @@ def test_empty_teacher_rows(hard):
     check(logits, idx, top, targets, temperature=2.0)
 
 
+@pytest.mark.parametrize("hard", [False, True])
+@pytest.mark.parametrize("k", [5, 64])
+def test_empty_teacher_rows_among_many(k, hard):
+    """Batches of 4096 rows and more share a warp between teacher rows: rows without a teacher,
+    with NaN, ids out of range or ids standing twice lie beside ordinary ones."""
+    logits, idx, top, targets = inputs(4200, 96, k, FP, seed=15, hard=hard)
+    idx[5::3] = -1
+    top[7::11] = -float("inf")
+    idx[8::13, 0] = idx[8::13, 1].clamp(min=0)
+    idx[8::13, 1] = idx[8::13, 0]
+    check(logits, idx, top, targets)
+    idx[100, 0] = 7
+    top[100, 0] = float("nan")
+    idx[201, 0] = 96
+    if hard:
+        targets[100] = targets[201] = 3
+    xg = logits.cuda().requires_grad_(True)
+    loss = fk.fused_distillation_loss(xg, idx.cuda(), top.cuda(),
+                                      None if targets is None else targets.cuda())
+    loss.backward()
+    assert torch.isnan(loss) and last_distillation_error() == 1
+    assert torch.isnan(xg.grad[201]).all() and torch.isnan(xg.grad[100]).any()
+    rest = [i for i in range(4200) if i not in (100, 201)]
+    assert torch.isfinite(xg.grad[rest]).all()
+
+
 def test_nothing_counts():
     logits, idx, top, targets = inputs(4, 60, 3, BF, seed=4)
     loss, grad = check(logits, idx, top, torch.full_like(targets, -100))
