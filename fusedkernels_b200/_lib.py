@@ -37,6 +37,7 @@ SIGNATURES: dict[str, list] = {
                            _sz, _i64, _i64, _i32, _vp],
     "fk_add_rmsnorm_quant": [_vp, _i64, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _i64,
                              _i64, _f32, _i32, _vp],
+    "fk_grad_rescale": [_vp, _i64, _i64, _i64, _vp, _f32, _i32, _vp],
     "fk_moe_balance_workspace_size": [C.POINTER(_sz)],
     "fk_moe_balance": [_vp, _i64, _vp, _vp, _i64, _i32, _i32, _f32, _f32, _vp, _vp, _vp, _vp, _sz,
                        _i32, _vp],
@@ -248,12 +249,10 @@ def hand_over_gradient(ctx, grad_output: torch.Tensor) -> torch.Tensor:
                            "pass: compute the loss again for another one")
     ctx.grad = None
     go = grad_output if grad_output.dtype == torch.float32 else grad_output.to(torch.float32)
-    if ctx.loss_scale != 1.0:
-        go = go / ctx.loss_scale
     rows, cols = grad.shape
     with on_device(grad):
-        call("fk_ce_bwd_scale", grad.data_ptr(), max(grad.stride(0), cols), rows, cols,
-             go.data_ptr(), _DTYPE_CODES[grad.dtype], stream_of(grad))
+        call("fk_grad_rescale", grad.data_ptr(), max(grad.stride(0), cols), rows, cols,
+             go.data_ptr(), ctx.loss_scale, _DTYPE_CODES[grad.dtype], stream_of(grad))
     return grad.detach()
 
 

@@ -874,9 +874,8 @@ int rows_mode(const T* lp, int64_t ls, T* gp, int64_t gs, const RowArgs& a, cuda
   constexpr bool keep = sizeof(T) == 4 && M != kTwo;
   if (per <= 128) return launch_rows<T, M, true, 128, 1, 8>(lp, ls, gp, gs, lc, bytes, a, st);
   if (per <= 512) return launch_rows<T, M, keep, 128, 4, 8>(lp, ls, gp, gs, lc, bytes, a, st);
-  constexpr int ctas = sizeof(T) == 2 && M == kTwo ? 3 : 4;
-  if (per <= 2048) return launch_rows<T, M, keep, 128, 16, ctas>(lp, ls, gp, gs, lc, bytes, a, st);
-  return launch_rows<T, M, keep, 256, 16, ctas / 2>(lp, ls, gp, gs, lc, bytes, a, st);
+  if (per <= 2048) return launch_rows<T, M, keep, 128, 16, 4>(lp, ls, gp, gs, lc, bytes, a, st);
+  return launch_rows<T, M, keep, 256, 16, 2>(lp, ls, gp, gs, lc, bytes, a, st);
 }
 
 template <typename T>

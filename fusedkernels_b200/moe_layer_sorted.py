@@ -33,6 +33,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .moe_balance import fused_moe_balance_loss
 from .moe_layer import Expert
 from .moe_routing import fused_moe_route
 from .moe_routing_v2 import fused_moe_route_v2
@@ -288,19 +289,33 @@ class _SortedMoEFn(torch.autograd.Function):
 
 
 class FusedMoEMLPSorted(nn.Module):
+    """``balance_coef`` and ``z_coef`` (not in the reference; 0 leaves the layer as it was) ask
+    for the routing's balance loss: each forward then leaves ``balance_loss`` = balance_coef *
+    E sum_e f_e P_e + z_coef * mean(logsumexp^2) for the caller to add to its loss, and
+    ``expert_counts``, the tokens' slots per expert (int64 [E])."""
+
     def __init__(self, dim: int, hidden_dim: int, n_experts: int, k: int = 2,
-                 router_version: str = "v2"):
+                 router_version: str = "v2", balance_coef: float = 0.0, z_coef: float = 0.0):
         super().__init__()
+        assert balance_coef >= 0.0 and z_coef >= 0.0
+        assert balance_coef > 0.0 or z_coef == 0.0, "z_coef goes with a balance_coef"
         assert router_version in ("v1", "v2")
         self.dim = dim
         self.hidden_dim = hidden_dim
         self.n_experts = n_experts
         self.k = k
         self.router_version = router_version
+        self.balance_coef = balance_coef
+        self.z_coef = z_coef
+        self.balance_loss = None
+        self.expert_counts = None
         self.router = nn.Linear(dim, n_experts, bias=False)
         self.experts = nn.ModuleList([Expert(dim, hidden_dim) for _ in range(n_experts)])
         self.check_errors = False  # True: read the device error flags after each call (syncs)
         self._restack()
+
+    def __getstate__(self):  # what a forward left belongs to its graph, not to a copy
+        return dict(self.__dict__, balance_loss=None, expert_counts=None)
 
     # -- stacked expert storage ------------------------------------------------------
     def _expert_params(self):
@@ -362,5 +377,10 @@ class FusedMoEMLPSorted(nn.Module):
         router_logits = self.router(x_flat)
         route_fn = fused_moe_route_v2 if self.router_version == "v2" else fused_moe_route
         topk_weights, topk_idx = route_fn(router_logits, self.k)
+        if self.balance_coef > 0.0:
+            loss, self.expert_counts = fused_moe_balance_loss(
+                router_logits, topk_idx, z_coef=self.z_coef / self.balance_coef,
+                loss_scale=self.balance_coef)
+            self.balance_loss = loss * self.balance_coef
         out = _SortedMoEFn.apply(x_flat, topk_weights, topk_idx, self, *self._expert_params())
         return out.reshape(orig_shape)

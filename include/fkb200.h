@@ -191,7 +191,7 @@ FK_API int fk_ce_bwd_scale(void* grad, int64_t grad_row_stride, int64_t n_rows, 
  * part.  An id or target out of range sets *err_flag = 1 and makes that row's loss and
  * gradient NaN.  loss[0] is the mean over the counted rows (fixed-order sum), not scaled by
  * loss_scale.  grad may be NULL (loss only) or alias logits.  The gradient is for
- * grad_output == loss_scale; fk_ce_bwd_scale turns it into another one. */
+ * grad_output == loss_scale; fk_grad_rescale turns it into another one's. */
 FK_API int fk_distill_workspace_size(int64_t n_rows, int k, size_t* bytes);
 FK_API int fk_distill(const void* logits, int64_t row_stride, void* grad,
                       int64_t grad_row_stride, const int64_t* teacher_idx,
@@ -200,6 +200,12 @@ FK_API int fk_distill(const void* logits, int64_t row_stride, void* grad,
                       int64_t ignore_index, float temperature, float hard_weight,
                       float loss_scale, int dtype, float* loss, int* err_flag, void* workspace,
                       size_t workspace_bytes, void* stream);
+
+/* grad *= grad_output[0] / expected unless grad_output[0] == expected (decided on the device:
+ * the launch then leaves without touching grad).  For gradients written by a forward pass
+ * with loss_scale = expected.  grad: [rows, cols] with row stride. */
+FK_API int fk_grad_rescale(void* grad, int64_t row_stride, int64_t rows, int64_t cols,
+                           const float* grad_output, float expected, int dtype, void* stream);
 
 /* ---------------------------------------------------------------- MoE balance loss
  * No counterpart in the reference.  For the router's logits [n_rows, n_experts] (row stride

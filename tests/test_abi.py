@@ -161,3 +161,14 @@ def test_distill_argument_checks():
     assert run(hw=1.5) == 1 and run(hw=float("nan")) == 1 and run(dt=3) == 1 and run(tdt=-1) == 1
     assert run(ptr=None) == 1
     assert run(ws=None) == 4 and run(ws=8) == 4 and run(size=16) == 4
+
+
+def test_grad_rescale_argument_checks():
+    lib = _lib.load()
+
+    def run(ptr=16, stride=8, rows=4, cols=8, expected=1.0, dt=0):
+        return lib.fk_grad_rescale(ptr, stride, rows, cols, ptr, expected, dt, None)
+
+    assert run(ptr=None) == 1 and run(stride=7) == 1 and run(rows=-1) == 1 and run(dt=5) == 1
+    assert run(expected=0.0) == 1 and run(expected=float("nan")) == 1
+    assert run(rows=0) == 0 and run(cols=0) == 0
