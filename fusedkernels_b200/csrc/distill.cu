@@ -255,6 +255,8 @@ struct RowArgs {
   int n_cols;
   int64_t n_rows;
   float temperature, inv_t, hard_weight, loss_scale;
+  float inv_p;   // kPowers: 1 / P
+  bool q2, p4;   // Q = 2, P = 4 (else 1, 3)
 };
 
 // Rows that count, at least 1 (whole warps call; all threads return the same number).
@@ -444,9 +446,11 @@ __device__ __forceinline__ float warp_redux_max(float v) {
   return r;
 }
 
-// What a row needs: softmax at one temperature, at two (the soft part's and 1), or at 2 and 1,
-// where exp(d) is the square of exp(d / 2).
-enum Mode { kOne, kTwo, kSquare };
+// What a row needs: softmax at one temperature, or at two (the soft part's, T, and 1).  Where T
+// is a ratio of small numbers P / Q, one exponential b = exp(d / P) gives both: b^Q = exp(d / T)
+// and b^P = exp(d).  kSquare is T = 2, kPowers T = 3, 4 and 3 / 2 (at 4096 x 128256 bf16: one
+// temperature 362 us, T = 2 386, two exponentials per logit 722).
+enum Mode { kOne, kTwo, kSquare, kPowers };
 
 // (maximum, sum exp((x - max) / T), sum exp(x - max)) of a set of logits.
 struct Stat {
@@ -530,7 +534,13 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
   ptx::wait_for_previous_kernel();  // the logits are older; the rest is the teacher kernel's
   const float inv_n = 1.0f / count_valid(a);
   const float inv_t = a.inv_t;
-  const float ct_row = inv_t * kLog2e;  // exponent of 2 per unit of logit
+  const float inv_b = M == kPowers ? a.inv_p : inv_t;  // b = exp(d * inv_b)
+  const float ct_row = inv_b * kLog2e;                  // exponent of 2 per unit of logit
+  auto powers = [&](float b, float& f, float& f1) {
+    const float b2 = b * b;
+    f = a.q2 ? b2 : b;
+    f1 = b2 * (a.p4 ? b2 : b);
+  };
   const bool same_slice = lstride % VN == 0;  // every row has the first row's offset
   const bool lists = warp * 32 < a.list;      // this warp has listed elements to handle
   bool ok = true;
@@ -627,14 +637,17 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
         if constexpr (M == kTwo) f1 = ex2f(fmaf(x, kLog2e, nb_1));
       } else {
         const float d = x - base;
-        f = exp2_of(d * inv_t);
+        f = exp2_of(d * inv_b);
         if constexpr (M == kTwo) f1 = exp2_of(d);
       }
       if constexpr (M == kSquare) f1 = f * f;
     };
     float2 e[KEEP ? KP : 1][NP], e1[KEEP && M == kTwo ? KP : 1][NP];
     float2 z = make_float2(0.f, 0.f), z1 = z;
-    if (xs_at >= 0) exp_one(xs, z.x, z1.x);
+    if (xs_at >= 0) {
+      exp_one(xs, z.x, z1.x);
+      if constexpr (M == kPowers) powers(z.x, z.x, z1.x);
+    }
 #pragma unroll
     for (int u = 0; u < KP; ++u)
 #pragma unroll
@@ -644,13 +657,26 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
         if constexpr (sizeof(T) == 2 && M != kTwo) {
           const float2 t = __ffma2_rn(x, make_float2(ct_row, ct_row), make_float2(nb_t, nb_t));
           f = make_float2(ex2f(t.x), ex2f(t.y));
-          z = __fadd2_rn(z, f);
-          if constexpr (M == kSquare) z1 = __ffma2_rn(f, f, z1);
+          if constexpr (M == kPowers) {
+            float2 g;
+            powers(f.x, g.x, f1.x);
+            powers(f.y, g.y, f1.y);
+            z = __fadd2_rn(z, g);
+            z1 = __fadd2_rn(z1, f1);
+          } else {
+            z = __fadd2_rn(z, f);
+            if constexpr (M == kSquare) z1 = __ffma2_rn(f, f, z1);
+          }
         } else {
           exp_one(x.x, f.x, f1.x);
           exp_one(x.y, f.y, f1.y);
-          z.x += f.x;
-          z.y += f.y;
+          float2 g = f;
+          if constexpr (M == kPowers) {
+            powers(f.x, g.x, f1.x);
+            powers(f.y, g.y, f1.y);
+          }
+          z.x += g.x;
+          z.y += g.y;
           if constexpr (M != kOne) {
             z1.x += f1.x;
             z1.y += f1.y;
@@ -703,20 +729,28 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
       } else {
         // 16 bits: the factor k / z goes into the exponent.
         const float ot = fmaf(-st.m, ct_row, __log2f(kt)), o1 = fmaf(-st.m, kLog2e, __log2f(k1));
+        // wt exp(d / T) and, where one exponential gives both, + w1 exp(d).
+        auto both = [&](float b, float wt, float w1) {
+          if constexpr (M == kPowers) {
+            float f, f1;
+            powers(b, f, f1);
+            return fmaf(f1, w1, f * wt);
+          }
+          return b * (M == kSquare ? fmaf(b, w1, wt) : wt);
+        };
         auto dense = [&](float x) {
           float g;
           if constexpr (sizeof(T) == 2) {
-            if constexpr (M == kSquare) {  // k1 e^2 + kt e
-              const float f = ex2f(fmaf(x, ct_row, -st.m * ct_row));
-              g = f * fmaf(f, k1, kt);
+            if constexpr (M == kSquare || M == kPowers) {
+              const float b = ex2f(fmaf(x, ct_row, -st.m * ct_row));
+              g = both(b, kt, k1);
             } else {
               g = ex2f(fmaf(x, ct_row, ot));
               if constexpr (M == kTwo) g += ex2f(fmaf(x, kLog2e, o1));
             }
           } else {
             const float d = x - st.m;
-            const float f = exp2_of(d * inv_t);
-            g = f * (M == kSquare ? fmaf(f, k1, kt) : kt);
+            g = both(exp2_of(d * inv_b), kt, k1);
             if constexpr (M == kTwo) g = fmaf(exp2_of(d), k1, g);
           }
           return g;
@@ -735,11 +769,7 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
           for (int k = 0; k < NP; ++k) {
             if constexpr (KEEP) {
               const float2 f = e[u][k];
-              float2 g;
-              if constexpr (M == kSquare)
-                g = make_float2(f.x * fmaf(f.x, f1, ft), f.y * fmaf(f.y, f1, ft));
-              else
-                g = make_float2(f.x * ft, f.y * ft);
+              float2 g = make_float2(both(f.x, ft, f1), both(f.y, ft, f1));
               if constexpr (M == kTwo)
                 g = make_float2(fmaf(e1[u][k].x, f1, g.x), fmaf(e1[u][k].y, f1, g.y));
               o.p[k].set(g);
@@ -871,7 +901,7 @@ int rows_mode(const T* lp, int64_t ls, T* gp, int64_t gs, const RowArgs& a, cuda
   while (lc < 3 && (a.n_rows << lc) < num_sms() && (packets >> lc) > 512) ++lc;
   const int64_t per = (packets + ((int64_t)1 << lc) - 1) >> lc;
   const int bytes = (int)(per < 1 ? 16 : per * 16);
-  constexpr bool keep = sizeof(T) == 4 && M != kTwo;
+  constexpr bool keep = sizeof(T) == 4 && (M == kOne || M == kSquare);
   if (per <= 128) return launch_rows<T, M, true, 128, 1, 8>(lp, ls, gp, gs, lc, bytes, a, st);
   if (per <= 512) return launch_rows<T, M, keep, 128, 4, 8>(lp, ls, gp, gs, lc, bytes, a, st);
   if (per <= 2048) return launch_rows<T, M, keep, 128, 16, 4>(lp, ls, gp, gs, lc, bytes, a, st);
@@ -892,6 +922,10 @@ int rows_t(const void* logits, int64_t ls, void* grad, int64_t gs, const RowArgs
     if (b.temperature == 1.f || a.hard_weight == 0.f)
       return rows_mode<T, kOne>(lp, ls, gp, gs, b, st);
     if (b.temperature == 2.f) return rows_mode<T, kSquare>(lp, ls, gp, gs, b, st);
+    b.q2 = b.temperature == 1.5f;
+    b.p4 = b.temperature == 4.f;
+    b.inv_p = b.p4 ? 0.25f : 1.0f / 3.0f;
+    if (b.q2 || b.p4 || b.temperature == 3.f) return rows_mode<T, kPowers>(lp, ls, gp, gs, b, st);
     return rows_mode<T, kTwo>(lp, ls, gp, gs, b, st);
   }
   const int64_t most = (int64_t)num_sms() * 8;
@@ -983,6 +1017,8 @@ extern "C" int fk_distill(const void* logits, int64_t row_stride, void* grad,
   a.n_rows = n_rows;
   a.temperature = temperature;
   a.inv_t = 1.0f / temperature;
+  a.inv_p = 1.f;
+  a.q2 = a.p4 = false;
   a.hard_weight = targets ? hard_weight : 0.f;
   a.loss_scale = loss_scale;
   FK_DISPATCH_DTYPE(dtype, s = fk::rows_t<scalar_t>(logits, row_stride, grad, grad_row_stride, a,

@@ -55,7 +55,7 @@ def check(logits, idx, top, targets, temperature=1.0, hard_weight=0.5, scale=1.0
 
 @pytest.mark.parametrize("dtype", [FP, BF, HF])
 @pytest.mark.parametrize("hard", [False, True])
-@pytest.mark.parametrize("temperature", [1.0, 2.0, 1.5])
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 1.5, 3.0, 4.0, 2.3, 0.7])
 @pytest.mark.parametrize("n,v,k", [(1, 1, 1), (1, 50, 3), (5, 7, 7), (40, 1000, 16),
                                    (9, 4099, 33), (3, 32000, 64), (2, 50257, 100)])
 def test_matches_64_bits(n, v, k, temperature, hard, dtype):
