@@ -60,20 +60,23 @@ __device__ __forceinline__ uint8_t to_e4m3(float v) {
 
 // ------------------------------------------------------------------ 16-byte chunks ------
 // A chunk is 16 bytes of x (VN elements) and the same elements of the residual: one 16-byte
-// load, or two where the residual is fp32 beside 16-bit x.
+// load, or two where the residual is fp32 beside 16-bit x.  A chunk of one element (VN = 1)
+// serves rows of any width and alignment.
 template <typename R, int VN>
 struct Chunk {
   static constexpr int N16 = VN * (int)sizeof(R) / 16;
   union {
-    uint4 u[N16];
+    uint4 u[N16 > 0 ? N16 : 1];
     R e[VN];
   };
   __device__ __forceinline__ Chunk() {}
   __device__ __forceinline__ void load(const R* p) {
+    if constexpr (VN == 1) e[0] = *p;
 #pragma unroll
     for (int i = 0; i < N16; ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
   }
   __device__ __forceinline__ void store(R* p) const {
+    if constexpr (VN == 1) *p = e[0];
 #pragma unroll
     for (int i = 0; i < N16; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, u[i]);
   }
@@ -82,6 +85,10 @@ struct Chunk {
 // VN weights from column c on (a multiple of VN), in fp32; they stay in L1 from row to row.
 template <int VN>
 __device__ __forceinline__ void load_weights(const void* w, int wd, int c, float (&out)[VN]) {
+  if constexpr (VN == 1) {
+    out[0] = load_wd(w, wd, c);
+    return;
+  }
   if (wd == FK_F32) {
 #pragma unroll
     for (int i = 0; i < VN; i += 4) {
@@ -135,14 +142,14 @@ constexpr int fwd_groups(int tpr) { return tpr <= 32 ? 256 / tpr : 1; }
 // threads take a row, thread t its chunks t, t + TPR, ...: every load of the row is in flight
 // before the first is used, the sum h stays in registers, and as the rows are independent the
 // SM hides one CTA's reduction under the others' loads.
-template <typename T, typename R, int TPR, int CPT, bool QUANT, bool BLOCK>
+template <typename T, typename R, int VN, int TPR, int CPT, bool QUANT, bool BLOCK>
 __global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR) add_rmsnorm_rows(
     const T* __restrict__ x, int64_t xs, const R* __restrict__ r, int64_t rs,
     const void* __restrict__ w, int wd, T* __restrict__ y, uint8_t* __restrict__ q,
     float* __restrict__ scales, R* __restrict__ h, float* __restrict__ rstd, int64_t rows,
     int cols, float eps) {
-  constexpr int VN = 16 / (int)sizeof(T);
   __shared__ float red[2][32];
+  __shared__ float group_max[VN == 1 && BLOCK ? CPT : 1][32];  // by warps
   const int t = threadIdx.x % TPR;
   const int64_t row0 = (int64_t)blockIdx.x * fwd_groups(TPR) + threadIdx.x / TPR;
   const bool there = TPR > 32 || row0 < rows;
@@ -208,20 +215,45 @@ __global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR) add_rmsnorm_rows(
     auto put = [&](int u, const float (&y)[VN], float inv) {
       const int c = t + u * TPR;
       if (c >= chunks || !there) return;
-      uint32_t o[VN / 4];
+      uint8_t* at = q + row * cols + c * VN;
+      if constexpr (VN == 1) {
+        *at = to_e4m3(y[0] * inv);
+        return;
+      }
+      uint32_t o[VN > 1 ? VN / 4 : 1];
 #pragma unroll
-      for (int k = 0; k < VN; k += 4) {
+      for (int k = 0; k + 3 < VN; k += 4) {
         const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[k] * inv, y[k + 1] * inv),
                                                      __NV_SATFINITE, __NV_E4M3);
         const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[k + 2] * inv, y[k + 3] * inv),
                                                      __NV_SATFINITE, __NV_E4M3);
         o[k / 4] = lo | hi << 16;
       }
-      uint8_t* at = q + row * cols + c * VN;
       if constexpr (VN == 8) __stcs(reinterpret_cast<uint2*>(at), make_uint2(o[0], o[1]));
-      else __stcs(reinterpret_cast<uint32_t*>(at), o[0]);
+      else if constexpr (VN == 4) __stcs(reinterpret_cast<uint32_t*>(at), o[0]);
     };
-    if constexpr (BLOCK) {
+    if constexpr (BLOCK && VN == 1) {
+      // 128 columns are four warps side by side: one exchange for all of the row's groups.
+      static_assert(TPR % 128 == 0, "groups of whole warps");
+      const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+      float y[CPT][VN];
+#pragma unroll
+      for (int u = 0; u < CPT; ++u) {
+        if (u * TPR >= cols) break;
+        const float m = warp_redux_max(values(u, y[u]));
+        if (lane == 0) group_max[u][warp] = m;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < CPT; ++u) {
+        if (u * TPR >= cols) break;
+        const float* g = &group_max[u][warp & ~3];
+        const float scale = scale_of(fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3])));
+        const int c = t + u * TPR;
+        if (t % 128 == 0 && c < cols) scales[row * ((cols + 127) / 128) + c / 128] = scale;
+        put(u, y[u], __fdividef(1.0f, scale));
+      }
+    } else if constexpr (BLOCK) {
       // The 128 / VN chunks of a group lie in neighbouring lanes (a row of 8 lanes is shorter
       // than a group).
       constexpr int kLanes = 128 / VN < TPR ? 128 / VN : TPR;
@@ -259,10 +291,11 @@ struct FwdArgs {
   float eps;
 };
 
-template <typename T, typename R, bool QUANT, bool BLOCK, int TPR, int CPT>
+template <typename T, typename R, bool QUANT, bool BLOCK, int TPR, int CPT,
+          int VN = 16 / (int)sizeof(T)>
 int launch_rows(const FwdArgs& a, cudaStream_t st) {
   const int64_t grid = (a.rows + fwd_groups(TPR) - 1) / fwd_groups(TPR);
-  add_rmsnorm_rows<T, R, TPR, CPT, QUANT, BLOCK><<<(unsigned)grid, TPR <= 32 ? 256 : TPR, 0, st>>>(
+  add_rmsnorm_rows<T, R, VN, TPR, CPT, QUANT, BLOCK><<<(unsigned)grid, TPR <= 32 ? 256 : TPR, 0, st>>>(
       static_cast<const T*>(a.x), a.xs, static_cast<const R*>(a.r), a.rs, a.w, a.wd,
       static_cast<T*>(a.y), static_cast<uint8_t*>(a.q), a.scales, static_cast<R*>(a.h), a.rstd,
       a.rows, (int)a.cols, a.eps);
@@ -296,6 +329,19 @@ int rows_chunked(const FwdArgs& a, cudaStream_t st) {
   if (chunks <= 768) return launch_rows<T, R, QUANT, BLOCK, 256, 3>(a, st);
   if (chunks <= 1024) return launch_rows<T, R, QUANT, BLOCK, 256, 4>(a, st);
   if (chunks <= 2048) return launch_rows<T, R, QUANT, BLOCK, 512, 4>(a, st);
+  return -1;
+}
+
+// The same with single elements, for rows that are not whole chunks; -1 where they are too long.
+template <typename T, typename R, bool QUANT, bool BLOCK>
+int rows_single(const FwdArgs& a, cudaStream_t st) {
+  if (a.rows >= (int64_t)1 << 31) return -1;
+  if (a.cols <= 128) return launch_rows<T, R, QUANT, BLOCK, 128, 1, 1>(a, st);
+  if (a.cols <= 512) return launch_rows<T, R, QUANT, BLOCK, 128, 4, 1>(a, st);
+  if (a.cols <= 1024) return launch_rows<T, R, QUANT, BLOCK, 128, 8, 1>(a, st);
+  if (a.cols <= 2048) return launch_rows<T, R, QUANT, BLOCK, 256, 8, 1>(a, st);
+  if (a.cols <= 4096) return launch_rows<T, R, QUANT, BLOCK, 512, 8, 1>(a, st);
+  if (a.cols <= 8192) return launch_rows<T, R, QUANT, BLOCK, 512, 16, 1>(a, st);
   return -1;
 }
 
@@ -582,242 +628,97 @@ int bwd_chunked(const BwdArgs& a, int* grid, cudaStream_t st) {
   return -1;
 }
 
-// ------------------------------------------------------------------ tiles ---------------
-// Contiguous rows of a width that is not whole chunks: 16 / sizeof(T) rows together are a
-// multiple of 16 bytes in every tensor, whatever the width.  A tile of some such rows comes to
-// shared memory by cp.async.bulk, a warp takes a row of it (single elements, no bank
-// conflicts), results go over the inputs and leave by bulk stores: memory sees whole lines
-// only.  The last rows, fewer than a unit, are copied element by element.
-//
-// Copies a tile's elements (whole: a multiple of 16 bytes, by the bulk unit).
-template <typename E>
-__device__ __forceinline__ void tile_in(E* dst, const E* src, int elements, bool whole,
-                                        uint64_t* bar) {
-  if (whole) {
-    if (threadIdx.x == 0) ptx::bulk_g2s(dst, src, (uint32_t)(elements * sizeof(E)), bar);
-  } else {
-    for (int i = threadIdx.x; i < elements; i += blockDim.x) dst[i] = src[i];
+// ------------------------------------------------------------------ backward, columns ---
+// Rows of any width, stride and alignment: thread t of the CTA has the columns t, t + THREADS,
+// ... as single elements, the next row's on their way while this one is worked on.
+template <typename T, typename R, int THREADS, int CPT>
+__global__ void __launch_bounds__(THREADS) add_rmsnorm_bwd_columns(BwdArgs a) {
+  __shared__ float red[2][32];
+  const int t = threadIdx.x;
+  const T* dy = static_cast<const T*>(a.dy);
+  const R *dh = static_cast<const R*>(a.dh), *h = static_cast<const R*>(a.h);
+  const float inv_cols = 1.0f / (float)a.cols;
+  float wv[CPT], acc[CPT];
+  T ndy[CPT];
+  R nh[CPT], ndh[CPT];
+  float ns = 0.f;
+#pragma unroll
+  for (int u = 0; u < CPT; ++u) {
+    const int c = t + u * THREADS;
+    acc[u] = 0.f;
+    wv[u] = c < a.cols ? load_wd(a.w, a.wd, c) : 0.f;
+    ndy[u] = Elt<T>::from_f(0.f);
+    nh[u] = ndh[u] = Elt<R>::from_f(0.f);
   }
-}
-template <typename E>
-__device__ __forceinline__ void tile_out(E* dst, const E* src, int elements, bool whole) {
-  if (whole) {
-    if (threadIdx.x == 0) ptx::bulk_s2g(dst, src, (uint32_t)(elements * sizeof(E)));
-  } else {
-    for (int i = threadIdx.x; i < elements; i += blockDim.x) dst[i] = src[i];
-  }
-}
-inline __host__ __device__ int align128(int n) { return (n + 127) / 128 * 128; }
-
-constexpr int kTileThreads = 256;
-
-// Forward (QUANT: the 8-bit form; q leaves as single bytes, 32 of a warp side by side).
-template <typename T, typename R, bool QUANT>
-__global__ void __launch_bounds__(kTileThreads) add_rmsnorm_tile(FwdArgs a, int tile_rows,
-                                                                 int block) {
-  constexpr int kUnit = 16 / (int)sizeof(T);
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ __align__(8) uint64_t full;
-  const int cols = (int)a.cols, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row0 = (int64_t)blockIdx.x * tile_rows;
-  const int n = (int)(a.rows - row0 < tile_rows ? a.rows - row0 : tile_rows);
-  const bool whole = n % kUnit == 0;
-  T* xt = reinterpret_cast<T*>(smem);
-  R* ht = reinterpret_cast<R*>(smem + align128(tile_rows * cols * (int)sizeof(T)));
-  if (threadIdx.x == 0) {
-    ptx::mbar_init(&full, 1);
-    ptx::fence_mbar_init();
-    ptx::fence_proxy_async_smem();
-    if (whole) ptx::mbar_arrive_expect_tx(&full, (uint32_t)(n * cols * (sizeof(T) + (a.r ? sizeof(R) : 0))));
-  }
-  tile_in(xt, static_cast<const T*>(a.x) + row0 * cols, n * cols, whole, &full);
-  if (a.r) tile_in(ht, static_cast<const R*>(a.r) + row0 * cols, n * cols, whole, &full);
-  __syncthreads();
-  // (A wait that runs out poisons the tile.)
-  const bool ok = !whole || ptx::mbar_wait(&full, 0, kPolls);
-  for (int i = warp; i < n; i += kTileThreads / 32) {
-    T* x = xt + i * cols;
-    R* h = ht + i * cols;
-    float ss = 0.f;
-#pragma unroll 4
-    for (int c = lane; c < cols; c += 32) {
-      float f = Elt<T>::to_f(x[c]);
-      if (a.r) {
-        const R hv = Elt<R>::from_f(f + Elt<R>::to_f(h[c]));
-        h[c] = hv;
-        f = Elt<R>::to_f(hv);
+  auto load = [&](int row) {
+    if (row >= a.rows) return;
+    ns = __ldg(a.rstd + row);
+    const T* pd = dy + row * a.dys;
+    const R *ph = h + (int64_t)row * a.cols, *pg = dh + row * a.dhs;
+#pragma unroll
+    for (int u = 0; u < CPT; ++u) {
+      const int c = t + u * THREADS;
+      if (c < a.cols) {
+        ndy[u] = pd[c];
+        nh[u] = ph[c];
+        if (dh) ndh[u] = pg[c];
       }
-      ss = fmaf(f, f, ss);
     }
-    float s = rsqrtf(warp_sum(ss) / (float)cols + a.eps);
-    if (!ok) s = __int_as_float(0x7fc00000);
-    if constexpr (!QUANT) {
-      if (lane == 0 && a.rstd) a.rstd[row0 + i] = s;
-#pragma unroll 4
-      for (int c = lane; c < cols; c += 32)
-        x[c] = Elt<T>::from_f(Elt<R>::to_f(h[c]) * s * load_wd(a.w, a.wd, c));
-    } else {
-      auto y = [&](int c) {
-        return (a.r ? Elt<R>::to_f(h[c]) : Elt<T>::to_f(x[c])) * s * load_wd(a.w, a.wd, c);
-      };
-      uint8_t* q = static_cast<uint8_t*>(a.q) + (row0 + i) * cols;
-      const int groups = (cols + block - 1) / block;
-      for (int g = 0; g < groups; ++g) {
-        const int c0 = g * block, c1 = c0 + block < cols ? c0 + block : cols;
-        float m = 0.f;
-        for (int c = c0 + lane; c < c1; c += 32) m = fmaxf(m, fabsf(y(c)));
-        const float scale = scale_of(warp_max(m)), inv = __fdividef(1.0f, scale);
-        if (lane == 0) a.scales[(row0 + i) * groups + g] = scale;
-        for (int c = c0 + lane; c < c1; c += 32) q[c] = to_e4m3(y(c) * inv);
+  };
+  const int step = gridDim.x;
+  int parity = 0;
+  load(blockIdx.x);
+  for (int row = blockIdx.x; row < a.rows; row += step, parity ^= 1) {
+    const float s = ns;
+    float d[CPT], hv[CPT], g[CPT], dot = 0.f;
+#pragma unroll
+    for (int u = 0; u < CPT; ++u) {
+      d[u] = Elt<T>::to_f(ndy[u]);
+      hv[u] = Elt<R>::to_f(nh[u]);
+      g[u] = Elt<R>::to_f(ndh[u]);
+      dot = fmaf(wv[u] * d[u], hv[u], dot);
+      acc[u] = fmaf(d[u] * hv[u], s, acc[u]);
+    }
+    load(row + step);
+    dot = row_reduce<THREADS, false>(dot, red[parity]);
+    const float c2 = s * s * s * (dot * inv_cols);
+    T* px = static_cast<T*>(a.dx) + (int64_t)row * a.cols;
+    R* pr = static_cast<R*>(a.dr) + (int64_t)row * a.cols;
+#pragma unroll
+    for (int u = 0; u < CPT; ++u) {
+      const int c = t + u * THREADS;
+      if (c < a.cols) {
+        const float v = s * (wv[u] * d[u]) - hv[u] * c2 + g[u];
+        px[c] = Elt<T>::from_f(v);
+        if (sizeof(T) != sizeof(R)) pr[c] = Elt<R>::from_f(v);
       }
     }
   }
-  ptx::fence_proxy_async_smem();
-  __syncthreads();
-  if (!QUANT) tile_out(static_cast<T*>(a.y) + row0 * cols, xt, n * cols, whole);
-  if (a.r) tile_out(static_cast<R*>(a.h) + row0 * cols, ht, n * cols, whole);
-  if (threadIdx.x == 0) {
-    ptx::bulk_commit();
-    ptx::bulk_wait_read();
+#pragma unroll
+  for (int u = 0; u < CPT; ++u) {
+    const int c = t + u * THREADS;
+    if (c < a.cols) a.part[(int64_t)blockIdx.x * a.cols + c] = acc[u];
   }
 }
 
-// Backward: persistent CTAs over the tiles.  Warps form the rows' dots, then threads go down
-// the tile's columns: gradient over dy and h, and the column's part of dw, which is kept in
-// shared memory for the CTA's tiles.
-template <typename T, typename R>
-__global__ void __launch_bounds__(kTileThreads) add_rmsnorm_bwd_tile(BwdArgs a, int tile_rows) {
-  constexpr int kUnit = 16 / (int)sizeof(T);
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ __align__(8) uint64_t full;
-  const int cols = a.cols, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int tb = align128(tile_rows * cols * (int)sizeof(T));
-  const int rb = align128(tile_rows * cols * (int)sizeof(R));
-  T* dyt = reinterpret_cast<T*>(smem);
-  R* ht = reinterpret_cast<R*>(smem + tb);
-  R* dht = reinterpret_cast<R*>(smem + tb + rb);
-  float* acc = reinterpret_cast<float*>(smem + tb + (a.dh ? 2 : 1) * rb);  // [cols]
-  float2* coef = reinterpret_cast<float2*>(acc + (cols + 1) / 2 * 2);      // [tile_rows] (s, c2)
-  for (int c = threadIdx.x; c < cols; c += kTileThreads) acc[c] = 0.f;
-  if (threadIdx.x == 0) {
-    ptx::mbar_init(&full, 1);
-    ptx::fence_mbar_init();
-  }
-  __syncthreads();
-  const float inv_cols = 1.0f / (float)cols;
-  bool ok = true;
-  int phase = 0;
-  for (int row0 = blockIdx.x * tile_rows; row0 < a.rows; row0 += gridDim.x * tile_rows) {
-    const int n = a.rows - row0 < tile_rows ? a.rows - row0 : tile_rows, count = n * cols;
-    const bool whole = n % kUnit == 0;
-    const int64_t at = (int64_t)row0 * cols;
-    if (threadIdx.x == 0 && whole) {
-      ptx::fence_proxy_async_smem();
-      ptx::mbar_arrive_expect_tx(&full, (uint32_t)(count * (sizeof(T) + (a.dh ? 2 : 1) * sizeof(R))));
-    }
-    tile_in(dyt, static_cast<const T*>(a.dy) + at, count, whole, &full);
-    tile_in(ht, static_cast<const R*>(a.h) + at, count, whole, &full);
-    if (a.dh) tile_in(dht, static_cast<const R*>(a.dh) + at, count, whole, &full);
-    if (whole) {
-      ok = ptx::mbar_wait(&full, (uint32_t)phase, ok ? kPolls : 1u) && ok;
-      phase ^= 1;
-    } else {
-      __syncthreads();
-    }
-    for (int i = warp; i < n; i += kTileThreads / 32) {
-      const T* dy = dyt + i * cols;
-      const R* h = ht + i * cols;
-      float dot = 0.f;
-#pragma unroll 4
-      for (int c = lane; c < cols; c += 32)
-        dot = fmaf(load_wd(a.w, a.wd, c) * Elt<T>::to_f(dy[c]), Elt<R>::to_f(h[c]), dot);
-      dot = warp_sum(dot);
-      if (lane == 0) {
-        const float s = a.rstd[row0 + i];
-        coef[i] = make_float2(s, ok ? s * s * s * (dot * inv_cols) : __int_as_float(0x7fc00000));
-      }
-    }
-    __syncthreads();
-    for (int c = threadIdx.x; c < cols; c += kTileThreads) {
-      const float w = load_wd(a.w, a.wd, c);
-      float sum = 0.f;
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float2 k = coef[i];
-        const float d = Elt<T>::to_f(dyt[i * cols + c]), h = Elt<R>::to_f(ht[i * cols + c]);
-        float g = k.x * (w * d) - h * k.y;
-        if (a.dh) g += Elt<R>::to_f(dht[i * cols + c]);
-        sum = fmaf(d * h, k.x, sum);
-        dyt[i * cols + c] = Elt<T>::from_f(g);
-        if (sizeof(T) != sizeof(R)) ht[i * cols + c] = Elt<R>::from_f(g);
-      }
-      acc[c] += sum;  // a column is one thread's
-    }
-    ptx::fence_proxy_async_smem();
-    __syncthreads();
-    tile_out(static_cast<T*>(a.dx) + at, dyt, count, whole);
-    if (sizeof(T) != sizeof(R)) tile_out(static_cast<R*>(a.dr) + at, ht, count, whole);
-    if (threadIdx.x == 0) {
-      ptx::bulk_commit();
-      ptx::bulk_wait_read();
-    }
-    __syncthreads();  // the tile is free again
-  }
-  for (int c = threadIdx.x; c < cols; c += kTileThreads)
-    a.part[(int64_t)blockIdx.x * cols + c] = acc[c];
-}
-
-// Rows of a tile: units of 16 / sizeof(T) rows, about 32 KB of them, fewer where the rows are
-// too few for four tiles per SM; 0 where one unit does not fit `most` bytes.
-template <typename T>
-int tile_rows_for(int64_t rows, int64_t cols, int bytes_per_element, int most) {
-  constexpr int kUnit = 16 / (int)sizeof(T);
-  const int64_t unit = kUnit * cols * bytes_per_element;
-  if (unit + 1024 > most) return 0;
-  int64_t units = 32 * 1024 / unit;
-  const int64_t share = rows / ((int64_t)num_sms() * 4 * kUnit);
-  if (units > share) units = share;
-  if (units > 16) units = 16;
-  return kUnit * (int)(units < 1 ? 1 : units);
-}
-constexpr int kTileSmem = 222 * 1024;
-
-// Runs the tile kernel where the rows are contiguous and a unit of them fits; -1 elsewhere.
-template <typename T, typename R, bool QUANT>
-int fwd_tiled(const FwdArgs& a, int64_t block, cudaStream_t st) {
-  if (a.xs != a.cols || (a.r && a.rs != a.cols) || !aligned16(a.x) || !aligned16(a.r) ||
-      !aligned16(a.y) || !aligned16(a.h) || a.cols > 16384 || a.rows >= (int64_t)1 << 31)
-    return -1;
-  const int n = tile_rows_for<T>(a.rows, a.cols, (int)sizeof(T) + (a.r ? (int)sizeof(R) : 0),
-                                 kTileSmem);
-  if (n == 0) return -1;
-  constexpr auto kern = add_rmsnorm_tile<T, R, QUANT>;
-  allow_shared_memory<kern>(1024);
-  const int smem = align128(n * (int)a.cols * (int)sizeof(T)) +
-                   (a.r ? align128(n * (int)a.cols * (int)sizeof(R)) : 0);
-  const int64_t grid = (a.rows + n - 1) / n;
-  kern<<<(unsigned)grid, kTileThreads, smem, st>>>(a, n, (int)block);
-  return launch_status(QUANT ? "fk_add_rmsnorm_quant" : "fk_add_rmsnorm_fwd");
-}
-
-template <typename T, typename R>
-int bwd_tiled(const BwdArgs& a, int* grid, cudaStream_t st) {
-  const int per = (int)sizeof(T) + (a.dh ? 2 : 1) * (int)sizeof(R);
-  if (a.dys != a.cols || (a.dh && a.dhs != a.cols) || !aligned16(a.dy) || !aligned16(a.dh) ||
-      !aligned16(a.h) || !aligned16(a.dx) || !aligned16(a.dr) || a.cols > 16384)
-    return -1;
-  const int n = tile_rows_for<T>(a.rows, a.cols, per, kTileSmem - a.cols * 4);
-  if (n == 0) return -1;
-  constexpr auto kern = add_rmsnorm_bwd_tile<T, R>;
-  allow_shared_memory<kern>(1024);
-  const int smem = align128(n * a.cols * (int)sizeof(T)) +
-                   (a.dh ? 2 : 1) * align128(n * a.cols * (int)sizeof(R)) + (a.cols + 1) / 2 * 8 +
-                   n * 8;
-  const int64_t want = ((int64_t)a.rows + n - 1) / n;
-  const int most = num_sms() * resident_ctas<kern>(kTileThreads, smem);
-  *grid = (int)(want < most ? want : most);
-  kern<<<*grid, kTileThreads, smem, st>>>(a, n);
+template <typename T, typename R, int THREADS, int CPT>
+int launch_bwd_columns(const BwdArgs& a, int* grid, cudaStream_t st) {
+  constexpr auto kern = add_rmsnorm_bwd_columns<T, R, THREADS, CPT>;
+  const int most = num_sms() * resident_ctas<kern>(THREADS, 0);
+  *grid = a.rows < most ? a.rows : most;
+  kern<<<*grid, THREADS, 0, st>>>(a);
   return launch_status("fk_add_rmsnorm_bwd");
+}
+
+template <typename T, typename R>
+int bwd_columns(const BwdArgs& a, int* grid, cudaStream_t st) {
+  if (a.cols <= 128) return launch_bwd_columns<T, R, 128, 1>(a, grid, st);
+  if (a.cols <= 512) return launch_bwd_columns<T, R, 128, 4>(a, grid, st);
+  if (a.cols <= 1024) return launch_bwd_columns<T, R, 128, 8>(a, grid, st);
+  if (a.cols <= 2048) return launch_bwd_columns<T, R, 256, 8>(a, grid, st);
+  if (a.cols <= 4096) return launch_bwd_columns<T, R, 512, 8>(a, grid, st);
+  if (a.cols <= 8192) return launch_bwd_columns<T, R, 512, 16>(a, grid, st);
+  return -1;
 }
 
 // ------------------------------------------------------------------ any shape -----------
@@ -944,7 +845,7 @@ int fwd_t(const void* x, int64_t xs, const void* r, int64_t rs, const void* w, i
           void* h, float* rstd, int64_t rows, int64_t cols, float eps, cudaStream_t st) {
   const FwdArgs a{x, r, w, y, nullptr, h, nullptr, rstd, xs, rs, rows, cols, wd, eps};
   int done = rows_chunked<T, R, false, false>(a, st);
-  if (done < 0) done = fwd_tiled<T, R, false>(a, 0, st);
+  if (done < 0) done = rows_single<T, R, false, false>(a, st);
   if (done >= 0) return done;
   add_rmsnorm_fwd_generic<T, R><<<row_grid(rows), 256, 0, st>>>(
       static_cast<const T*>(x), xs, static_cast<const R*>(r), rs, w, wd, static_cast<T*>(y),
@@ -960,7 +861,7 @@ int bwd_t(const void* dy, int64_t dys, const void* dh, int64_t dhs, const void* 
     const BwdArgs a{dy,  dh,  h,         w,         rstd, dx, dr,
                     part, dys, dhs, (int)rows, (int)cols, wd};
     int done = bwd_chunked<T, R>(a, grid, st);
-    if (done < 0) done = bwd_tiled<T, R>(a, grid, st);
+    if (done < 0) done = bwd_columns<T, R>(a, grid, st);
     if (done >= 0) return done;
   }
   *grid = row_grid(rows);
@@ -977,7 +878,9 @@ int quant_t(const void* x, int64_t xs, const void* r, int64_t rs, const void* w,
   const FwdArgs a{x, r, w, nullptr, q, h, scales, nullptr, xs, rs, rows, cols, wd, eps};
   int done = block == cols ? rows_chunked<T, R, true, false>(a, st)
                            : rows_chunked<T, R, true, true>(a, st);
-  if (done < 0) done = fwd_tiled<T, R, true>(a, block, st);
+  if (done < 0)
+    done = block == cols ? rows_single<T, R, true, false>(a, st)
+                         : rows_single<T, R, true, true>(a, st);
   if (done >= 0) return done;
   add_rmsnorm_quant_generic<T, R><<<row_grid(rows), 256, 0, st>>>(
       static_cast<const T*>(x), xs, static_cast<const R*>(r), rs, w, wd,

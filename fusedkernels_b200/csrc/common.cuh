@@ -102,6 +102,13 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// The same in one instruction (NaN is passed over, as by fmaxf).
+__device__ __forceinline__ float warp_redux_max(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // Sigmoid for the elementwise kernels.  16-bit element types use the fast exponential
 // and reciprocal (their outputs round to 8/11 mantissa bits); fp32 uses expf and IEEE
 // division.

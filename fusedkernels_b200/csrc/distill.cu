@@ -440,12 +440,6 @@ union PairPacket {
   __device__ __forceinline__ PairPacket() {}
 };
 
-__device__ __forceinline__ float warp_redux_max(float v) {
-  float r;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
-
 // What a row needs: softmax at one temperature, or at two (the soft part's, T, and 1).  Where T
 // is a ratio of small numbers P / Q, one exponential b = exp(d / P) gives both: b^Q = exp(d / T)
 // and b^P = exp(d).  kSquare is T = 2, kPowers T = 3, 4 and 3 / 2 (at 4096 x 128256 bf16: one

@@ -80,8 +80,7 @@ def test_many_rows(types):
 @pytest.mark.parametrize("types", TYPES, ids=str)
 @pytest.mark.parametrize("shape", [(10007, 33), (20005, 130), (9, 2001), (17, 7001)], ids=str)
 def test_odd_widths(shape, types):
-    """Widths that are not whole 16-byte packets: many short rows, rows left over at the end,
-    rows too long to be gathered in shared memory."""
+    """Widths that are not whole 16-byte packets: many short rows, long rows."""
     x, r, w, dy, dh = inputs(shape, *types, FP, seed=30 + shape[1])
     check(x, r, w, dy, dh, *leaves(x, r, w))
     check(x, r, w, dy, None, *leaves(x, r, w))
