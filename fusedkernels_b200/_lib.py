@@ -228,13 +228,27 @@ def rows_of(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int]:
     return t, max(t.stride(0), cols)  # a tensor of one row may report any stride
 
 
-def once_differentiable(fn):
-    """torch's once_differentiable, without its cost where no graph of the backward pass is
-    wanted (grad mode is off there)."""
-    guarded = torch.autograd.function.once_differentiable(fn)
+class _NoSecondDerivative(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, _anchor, *grads):
+        return tuple(None if g is None else g.view_as(g) for g in grads)
 
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("this operator has no second derivative: its backward pass is "
+                           "once_differentiable")
+
+
+def once_differentiable(fn):
+    """For backward passes made of kernels: under create_graph the gradients come with a node
+    that raises when they are differentiated, whether grad_output asks for it or not."""
     def backward(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return fn(ctx, *grads)
+        with torch.no_grad():
+            out = fn(ctx, *grads)
+        out = out if isinstance(out, tuple) else (out,)
+        return _NoSecondDerivative.apply(torch.empty(0, requires_grad=True), *out)
 
     return backward
 

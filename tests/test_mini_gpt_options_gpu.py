@@ -145,3 +145,18 @@ def test_command_line():
     r = subprocess.run(cmd, cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
     assert "mode=fused" in r.stdout and "loss=nan" not in r.stdout
+
+
+def test_no_second_derivatives():
+    """A backward pass with create_graph gives the gradient; a derivative of it is refused."""
+    from fusedkernels_b200 import (fused_add_rms_norm, fused_distillation_loss,
+                                   fused_moe_balance_loss)
+    x = torch.randn(6, 32, device="cuda", requires_grad=True)
+    w = torch.ones(32, device="cuda")
+    idx = torch.arange(12, device="cuda").view(6, 2) % 32
+    top = torch.randn(6, 2, device="cuda")
+    for loss in (fused_add_rms_norm(x, x.detach(), w)[0].sum(), fused_moe_balance_loss(x, idx)[0],
+                 fused_distillation_loss(x, idx, top)):
+        (g,) = torch.autograd.grad(loss, x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.square().sum().backward()
