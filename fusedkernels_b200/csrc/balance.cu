@@ -508,6 +508,7 @@ extern "C" int fk_moe_balance(const void* logits, int64_t row_stride, const int6
                "fk_moe_balance: nearly 2^31 slots or more");
   FK_CHECK_ARG(row_stride >= n_experts, "fk_moe_balance: stride < n_experts");
   FK_CHECK_ARG(fk::valid_dtype(dtype), "fk_moe_balance: bad dtype code %d", dtype);
+  FK_CHECK_ARG(loss_scale > 0.f && loss_scale < INFINITY, "fk_moe_balance: loss_scale must be > 0");
   FK_CHECK_ARG(counts && loss, "fk_moe_balance: null pointer");
   FK_CHECK_ARG(n_rows == 0 || (logits && (idx || k == 0)), "fk_moe_balance: null pointer");
   if (workspace == nullptr || workspace_bytes < fk::ws_bytes() || !fk::aligned16(workspace))

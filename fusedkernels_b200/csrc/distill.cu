@@ -980,6 +980,7 @@ extern "C" int fk_distill(const void* logits, int64_t row_stride, void* grad,
                "fk_distill: stride < n_cols");
   FK_CHECK_ARG(temperature > 0.f && temperature < INFINITY, "fk_distill: temperature must be > 0");
   FK_CHECK_ARG(hard_weight >= 0.f && hard_weight <= 1.f, "fk_distill: hard_weight outside [0, 1]");
+  FK_CHECK_ARG(loss_scale > 0.f && loss_scale < INFINITY, "fk_distill: loss_scale must be > 0");
   FK_CHECK_ARG(loss && err_flag, "fk_distill: null pointer");
   FK_CHECK_ARG(n_rows == 0 || (logits && teacher_idx && teacher_logits),
                "fk_distill: null pointer");

@@ -26,7 +26,6 @@ class _FusedDistillation(torch.autograd.Function):
         (teacher_idx, teacher_logits, targets, temperature, hard_weight, ignore_index,
          inplace_grad, loss_scale, want_grad) = args
         n_rows, n_cols = logits.shape
-        dev = logits.device
         x, stride = _lib.rows_of(logits, n_cols)
         idx = teacher_idx.to(torch.int64).contiguous()
         top = teacher_logits.contiguous()
@@ -37,12 +36,12 @@ class _FusedDistillation(torch.autograd.Function):
             if inplace_grad:
                 grad, grad_stride = x, stride
             else:
-                grad = torch.empty((n_rows, n_cols), dtype=x.dtype, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        err = torch.empty(1, dtype=torch.int32, device=dev)
+                grad = x.new_empty((n_rows, n_cols))
+        loss = x.new_empty((), dtype=torch.float32)
+        err = x.new_empty(1, dtype=torch.int32)
         k = idx.shape[1]
-        size = _lib.workspace_bytes("fk_distill_workspace_size", dev, n_rows, k)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        size = _lib.workspace_bytes("fk_distill_workspace_size", logits.device, n_rows, k)
+        ws = x.new_empty(size, dtype=torch.uint8)
         with _lib.on_device(logits):
             _lib.call("fk_distill", x.data_ptr(), stride, _lib.ptr(grad), grad_stride,
                       idx.data_ptr(), top.data_ptr(), _lib.dtype_code(top.dtype), k,
@@ -96,7 +95,8 @@ def fused_distillation_loss(logits: torch.Tensor, teacher_idx: torch.Tensor,
     if targets is not None:
         assert targets.shape == (n_rows,) and targets.device == logits.device
         assert not targets.is_floating_point()
-    assert temperature > 0.0 and 0.0 <= hard_weight <= 1.0 and loss_scale != 0.0
+    assert 0.0 < temperature < float("inf") and 0.0 <= hard_weight <= 1.0
+    assert 0.0 < loss_scale < float("inf")
     want_grad = torch.is_grad_enabled() and logits.requires_grad
     return _FusedDistillation.apply(logits, (teacher_idx, teacher_logits, targets,
                                              float(temperature), float(hard_weight),

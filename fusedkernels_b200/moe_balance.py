@@ -23,15 +23,14 @@ class _FusedMoEBalanceLoss(torch.autograd.Function):
     def forward(ctx, logits, args):
         topk_idx, token_mask, z_coef, loss_scale, want_grad = args
         n_rows, n_experts = logits.shape
-        dev = logits.device
         x, stride = _lib.rows_of(logits, n_experts)
         idx = topk_idx.to(torch.int64).contiguous()
         mask = None if token_mask is None else token_mask.contiguous()
-        grad = torch.empty((n_rows, n_experts), dtype=x.dtype, device=dev) if want_grad else None
-        counts = torch.empty(n_experts, dtype=torch.int64, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        size = _lib.workspace_bytes("fk_moe_balance_workspace_size", dev)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        grad = x.new_empty((n_rows, n_experts)) if want_grad else None
+        counts = x.new_empty(n_experts, dtype=torch.int64)
+        loss = x.new_empty((), dtype=torch.float32)
+        size = _lib.workspace_bytes("fk_moe_balance_workspace_size", logits.device)
+        ws = x.new_empty(size, dtype=torch.uint8)
         with _lib.on_device(logits):
             _lib.call("fk_moe_balance", x.data_ptr(), stride, idx.data_ptr(), _lib.ptr(mask),
                       n_rows, n_experts, idx.shape[1], z_coef, loss_scale, _lib.ptr(grad),
@@ -75,7 +74,7 @@ def fused_moe_balance_loss(router_logits: torch.Tensor, topk_idx: torch.Tensor,
     if token_mask is not None:
         assert token_mask.shape == (n_rows,) and token_mask.dtype == torch.bool
         assert token_mask.device == router_logits.device
-    assert loss_scale != 0.0
+    assert 0.0 < loss_scale < float("inf")
     want_grad = torch.is_grad_enabled() and router_logits.requires_grad
     return _FusedMoEBalanceLoss.apply(router_logits, (topk_idx, token_mask, float(z_coef),
                                                       float(loss_scale), want_grad))

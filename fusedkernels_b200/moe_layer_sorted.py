@@ -378,8 +378,10 @@ class FusedMoEMLPSorted(nn.Module):
         route_fn = fused_moe_route_v2 if self.router_version == "v2" else fused_moe_route
         topk_weights, topk_idx = route_fn(router_logits, self.k)
         if self.balance_coef > 0.0:
+            # fp16: its gradient stays in 32 bits until a loss scaler's factor has come
+            logits = router_logits.float() if x_flat.dtype == torch.float16 else router_logits
             loss, self.expert_counts = fused_moe_balance_loss(
-                router_logits, topk_idx, z_coef=self.z_coef / self.balance_coef,
+                logits, topk_idx, z_coef=self.z_coef / self.balance_coef,
                 loss_scale=self.balance_coef)
             self.balance_loss = loss * self.balance_coef
         out = _SortedMoEFn.apply(x_flat, topk_weights, topk_idx, self, *self._expert_params())

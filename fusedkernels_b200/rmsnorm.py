@@ -84,10 +84,9 @@ class _FusedAddRMSNormFn(torch.autograd.Function):
         x2, xs = _lib.rows_of(x, n_cols)
         r2, rs = _lib.rows_of(residual, n_cols)
         w = weight.contiguous()
-        dev = x.device
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
-        rstd = torch.empty(n_rows, dtype=torch.float32, device=dev) if save else None
+        y = x.new_empty(x.shape)  # (new_empty: the cheapest of torch's allocating calls)
+        h = residual.new_empty(x.shape)
+        rstd = x.new_empty(n_rows, dtype=torch.float32) if save else None
         with _lib.on_device(x):
             _lib.call("fk_add_rmsnorm_fwd", x2.data_ptr(), xs, r2.data_ptr(), rs,
                       _lib.dtype_code(h.dtype), w.data_ptr(), _lib.dtype_code(w.dtype),
@@ -112,15 +111,15 @@ class _FusedAddRMSNormFn(torch.autograd.Function):
             return (dh.to(ctx.x_dtype) if need_x else None, dh if need_r else None,
                     torch.zeros(ctx.weight_shape, dtype=w.dtype, device=w.device)
                     if need_w else None, None, None)
-        dev = h.device
         dy2, dys = _lib.rows_of(dy, n_cols)
         dh2, dhs = (None, 0) if dh is None else _lib.rows_of(dh, n_cols)
         n_rows = h.numel() // n_cols
-        dx = torch.empty(h.shape, dtype=ctx.x_dtype, device=dev)
-        dr = dx if h.dtype == ctx.x_dtype else torch.empty_like(h)
-        dw = torch.empty(ctx.weight_shape, dtype=w.dtype, device=dev)
-        size = _lib.workspace_bytes("fk_add_rmsnorm_bwd_workspace_size", dev, n_rows, n_cols)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        dx = h.new_empty(h.shape, dtype=ctx.x_dtype)
+        dr = dx if h.dtype == ctx.x_dtype else h.new_empty(h.shape)
+        dw = w.new_empty(ctx.weight_shape)
+        size = _lib.workspace_bytes("fk_add_rmsnorm_bwd_workspace_size", h.device, n_rows,
+                                    n_cols)
+        ws = h.new_empty(size, dtype=torch.uint8)
         with _lib.on_device(h):
             _lib.call("fk_add_rmsnorm_bwd", dy2.data_ptr(), dys, _lib.ptr(dh2), dhs, h.data_ptr(),
                       _lib.dtype_code(h.dtype), w.data_ptr(), _lib.dtype_code(w.dtype),
@@ -166,14 +165,13 @@ def fused_add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None,
     n_rows = x.numel() // n_cols
     x2, xs = _lib.rows_of(x, n_cols)
     w = weight.contiguous()
-    dev = x.device
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
     groups = 1 if block is None else -(-n_cols // block)
-    scales = torch.empty((*x.shape[:-1], groups), dtype=torch.float32, device=dev)
+    scales = x.new_empty((*x.shape[:-1], groups), dtype=torch.float32)
     r2, rs, h = None, 0, x
     if residual is not None:
         r2, rs = _lib.rows_of(residual, n_cols)
-        h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
+        h = residual.new_empty(x.shape)
     with _lib.on_device(x):
         _lib.call("fk_add_rmsnorm_quant", x2.data_ptr(), xs, _lib.ptr(r2), rs,
                   _lib.dtype_code(h.dtype), w.data_ptr(), _lib.dtype_code(w.dtype), q.data_ptr(),

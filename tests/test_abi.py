@@ -131,14 +131,14 @@ def test_balance_argument_checks():
     assert lib.fk_moe_balance_workspace_size(None) == 1
     assert lib.fk_moe_balance_workspace_size(ctypes.byref(n)) == 0 and n.value > 0
 
-    def run(stride=8, rows=4, e=8, k=2, dt=0, ptr=16, ws=16, size=1 << 30):
-        return lib.fk_moe_balance(ptr, stride, ptr, None, rows, e, k, 0.0, 1.0, None, ptr, ptr, ws,
+    def run(stride=8, rows=4, e=8, k=2, dt=0, ptr=16, ws=16, size=1 << 30, scale=1.0):
+        return lib.fk_moe_balance(ptr, stride, ptr, None, rows, e, k, 0.0, scale, None, ptr, ptr, ws,
                                   size, dt, None)
 
     assert run(e=257, stride=257) == 2 and b"257" in lib.fk_last_error()
     assert run(rows=-1) == 1 and run(e=0) == 1 and run(stride=7) == 1 and run(dt=3) == 1
     assert run(rows=1 << 30, k=2) == 1  # slots are counted in 32 bits
-    assert run(ptr=None) == 1
+    assert run(ptr=None) == 1 and run(scale=0.0) == 1 and run(scale=float("inf")) == 1
     assert run(ws=None) == 4 and run(ws=8) == 4 and run(size=16) == 4
 
 
@@ -150,14 +150,15 @@ def test_distill_argument_checks():
     assert lib.fk_distill_workspace_size(4, 2, ctypes.byref(n)) == 0 and n.value > 0
 
     def run(ptr=16, stride=8, grad=None, gstride=0, k=2, rows=4, cols=8, t=1.0, hw=0.5, dt=0, tdt=0,
-            ws=16, size=1 << 30):
+            ws=16, size=1 << 30, scale=1.0):
         return lib.fk_distill(ptr, stride, grad, gstride, ptr, ptr, tdt, k, None, rows, cols, -100, t,
-                              hw, 1.0, dt, ptr, ptr, ws, size, None)
+                              hw, scale, dt, ptr, ptr, ws, size, None)
 
     assert run(k=1025) == 2 and b"1025" in lib.fk_last_error()
     assert run(k=0) == 1 and run(rows=-1) == 1 and run(cols=0) == 1 and run(stride=7) == 1
     assert run(cols=1 << 31, stride=1 << 31) == 1 and run(grad=16, gstride=7) == 1
     assert run(t=0.0) == 1 and run(t=float("inf")) == 1 and run(t=float("nan")) == 1
+    assert run(scale=-1.0) == 1 and run(scale=float("nan")) == 1
     assert run(hw=1.5) == 1 and run(hw=float("nan")) == 1 and run(dt=3) == 1 and run(tdt=-1) == 1
     assert run(ptr=None) == 1
     assert run(ws=None) == 4 and run(ws=8) == 4 and run(size=16) == 4

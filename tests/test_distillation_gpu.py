@@ -278,7 +278,7 @@ def test_second_backward_raises_and_refusals():
                   ((x, idx, top, targets[:5]), {}), ((x, idx, top, targets.cpu()), {}),
                   ((x, idx, top, targets.float()), {}), ((x, idx, top), dict(temperature=0.0)),
                   ((x, idx, top, targets), dict(hard_weight=1.5)), ((x[0], idx, top), {}),
-                  ((x, idx, top), dict(loss_scale=0.0)), ((x.cpu(), idx.cpu(), top.cpu()), {})):
+                  ((x, idx, top), dict(loss_scale=-2.0)), ((x.cpu(), idx.cpu(), top.cpu()), {})):
         with pytest.raises(AssertionError):
             fk.fused_distillation_loss(*a, **kw)
     with pytest.raises(TypeError):

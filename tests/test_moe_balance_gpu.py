@@ -163,6 +163,8 @@ def test_second_backward_raises_and_refusals():
               (x[0], idx), (x.cpu(), idx.cpu())):
         with pytest.raises(AssertionError):
             fk.fused_moe_balance_loss(*a)
+    with pytest.raises(AssertionError):
+        fk.fused_moe_balance_loss(x, idx, loss_scale=0.0)
     with pytest.raises(TypeError):
         fk.fused_moe_balance_loss(x.double(), idx)
 
