@@ -192,6 +192,7 @@ FK_API int fk_ce_bwd_scale(void* grad, int64_t grad_row_stride, int64_t n_rows, 
  * gradient NaN.  loss[0] is the mean over the counted rows (fixed-order sum), not scaled by
  * loss_scale.  grad may be NULL (loss only) or alias logits.  The gradient is for
  * grad_output == loss_scale; fk_grad_rescale turns it into another one's. */
+/* Bytes of workspace (16-byte aligned, any contents) on the current device. */
 FK_API int fk_distill_workspace_size(int64_t n_rows, int k, size_t* bytes);
 FK_API int fk_distill(const void* logits, int64_t row_stride, void* grad,
                       int64_t grad_row_stride, const int64_t* teacher_idx,
@@ -218,6 +219,7 @@ FK_API int fk_grad_rescale(void* grad, int64_t row_stride, int64_t rows, int64_t
  * tokens get a zero gradient row.  grad [n_rows, n_experts] is contiguous, in the logits'
  * type (NULL: not wanted); loss is not scaled by loss_scale.  Integer counts and
  * fixed-order sums: the results do not depend on the order in which CTAs run. */
+/* Bytes of workspace (16-byte aligned, any contents) on the current device. */
 FK_API int fk_moe_balance_workspace_size(size_t* bytes);
 FK_API int fk_moe_balance(const void* logits, int64_t row_stride, const int64_t* idx,
                           const uint8_t* token_mask, int64_t n_rows, int n_experts, int k,

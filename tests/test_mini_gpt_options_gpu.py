@@ -138,6 +138,29 @@ def test_layer_attributes():
         FusedMoEMLPSorted(64, 64, 4, 2, z_coef=0.1)
 
 
+def test_fp16_layer_keeps_its_balance_gradient():
+    """The gradient of a mean over 4096 tokens, times 0.01, is below fp16's smallest step where
+    the loss scaler's factor comes after its rounding; here that factor comes first.  Bound: the
+    fp16 products of the router's backward (half_step 2^-11 per factor, three of them) over sums
+    of 4096 terms."""
+    layer = FusedMoEMLPSorted(64, 64, 8, 2, balance_coef=0.01).cuda().half()
+    x = torch.randn(4096, 64, device="cuda").half()
+    layer(x)
+    (layer.balance_loss * 65536.0).backward()
+    xd = x.double().cpu()
+    logits = (x @ layer.router.weight.T).detach().double().cpu()  # the layer's own, rounded
+    idx = logits.sort(dim=1, descending=True, stable=True).indices[:, :2]  # fp16 logits tie
+    assert torch.equal(torch.bincount(idx.reshape(-1), minlength=8), layer.expert_counts.cpu())
+    f = torch.bincount(idx.reshape(-1), minlength=8).double() / idx.numel()
+    p = torch.softmax(logits, 1)
+    dlogits = 65536 * 0.01 * 8 / 4096 * p * (f - (p * f).sum(1, keepdim=True))
+    want = dlogits.T @ xd
+    size = dlogits.abs().T @ xd.abs()
+    got = layer.router.weight.grad.double().cpu()
+    assert torch.count_nonzero(got) == got.numel()
+    assert ((got - want).abs() <= 3 * 2 ** -11 * size + 2 ** -24).all()
+
+
 def test_command_line():
     cmd = [sys.executable, "-m", "fusedkernels_b200.mini_gpt", "--steps", "2", "--warmup", "1",
            "--batch-size", "2", "--seq-len", "64", "--dim", "128", "--layers", "2",
