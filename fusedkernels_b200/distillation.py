@@ -19,39 +19,42 @@ MAX_SLOTS = 1024
 _last_err = None
 
 
+def _distill(logits, teacher_idx, teacher_logits, targets, temperature, hard_weight,
+             ignore_index, inplace_grad, loss_scale, want_grad):
+    """loss and (want_grad) the gradient of loss * loss_scale."""
+    global _last_err
+    n_rows, n_cols = logits.shape
+    x, stride = _lib.rows_of(logits, n_cols)
+    idx = teacher_idx.to(torch.int64).contiguous()
+    top = teacher_logits.contiguous()
+    if targets is not None:
+        targets = targets.to(torch.int64).contiguous()
+    grad, grad_stride = None, n_cols
+    if want_grad:
+        if inplace_grad:
+            grad, grad_stride = x, stride
+        else:
+            grad = x.new_empty((n_rows, n_cols))
+    loss = x.new_empty((), dtype=torch.float32)
+    err = x.new_empty(1, dtype=torch.int32)
+    k = idx.shape[1]
+    size = _lib.workspace_bytes("fk_distill_workspace_size", logits.device, n_rows, k)
+    ws = x.new_empty(size, dtype=torch.uint8)
+    with _lib.on_device(logits):
+        _lib.call("fk_distill", x.data_ptr(), stride, _lib.ptr(grad), grad_stride,
+                  idx.data_ptr(), top.data_ptr(), _lib.dtype_code(top.dtype), k,
+                  _lib.ptr(targets), n_rows, n_cols, ignore_index, temperature, hard_weight,
+                  loss_scale, _lib.dtype_code(x.dtype), loss.data_ptr(), err.data_ptr(),
+                  ws.data_ptr(), size, _lib.stream_of(logits))
+    _last_err = err
+    return loss, grad
+
+
 class _FusedDistillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, args):
-        global _last_err
-        (teacher_idx, teacher_logits, targets, temperature, hard_weight, ignore_index,
-         inplace_grad, loss_scale, want_grad) = args
-        n_rows, n_cols = logits.shape
-        x, stride = _lib.rows_of(logits, n_cols)
-        idx = teacher_idx.to(torch.int64).contiguous()
-        top = teacher_logits.contiguous()
-        if targets is not None:
-            targets = targets.to(torch.int64).contiguous()
-        grad, grad_stride = None, n_cols
-        if want_grad:
-            if inplace_grad:
-                grad, grad_stride = x, stride
-            else:
-                grad = x.new_empty((n_rows, n_cols))
-        loss = x.new_empty((), dtype=torch.float32)
-        err = x.new_empty(1, dtype=torch.int32)
-        k = idx.shape[1]
-        size = _lib.workspace_bytes("fk_distill_workspace_size", logits.device, n_rows, k)
-        ws = x.new_empty(size, dtype=torch.uint8)
-        with _lib.on_device(logits):
-            _lib.call("fk_distill", x.data_ptr(), stride, _lib.ptr(grad), grad_stride,
-                      idx.data_ptr(), top.data_ptr(), _lib.dtype_code(top.dtype), k,
-                      _lib.ptr(targets), n_rows, n_cols, ignore_index, temperature, hard_weight,
-                      loss_scale, _lib.dtype_code(x.dtype), loss.data_ptr(), err.data_ptr(),
-                      ws.data_ptr(), size, _lib.stream_of(logits))
-        _last_err = err
-        if want_grad:
-            ctx.grad = grad
-            ctx.loss_scale = loss_scale
+        loss, ctx.grad = _distill(logits, *args, True)
+        ctx.loss_scale = args[-1]
         return loss
 
     @staticmethod
@@ -97,11 +100,11 @@ def fused_distillation_loss(logits: torch.Tensor, teacher_idx: torch.Tensor,
         assert not targets.is_floating_point()
     assert 0.0 < temperature < float("inf") and 0.0 <= hard_weight <= 1.0
     assert 0.0 < loss_scale < float("inf")
-    want_grad = torch.is_grad_enabled() and logits.requires_grad
-    return _FusedDistillation.apply(logits, (teacher_idx, teacher_logits, targets,
-                                             float(temperature), float(hard_weight),
-                                             int(ignore_index), inplace_grad, float(loss_scale),
-                                             want_grad))
+    args = (teacher_idx, teacher_logits, targets, float(temperature), float(hard_weight),
+            int(ignore_index), inplace_grad, float(loss_scale))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _FusedDistillation.apply(logits, args)
+    return _distill(logits, *args, False)[0]
 
 
 def last_distillation_error() -> int:

@@ -18,29 +18,32 @@ from . import _lib
 from .moe_routing_v2 import MAX_EXPERTS
 
 
+def _balance(logits, topk_idx, token_mask, z_coef, loss_scale, want_grad):
+    """loss, counts and (want_grad) the gradient of loss * loss_scale."""
+    n_rows, n_experts = logits.shape
+    x, stride = _lib.rows_of(logits, n_experts)
+    idx = topk_idx.to(torch.int64).contiguous()
+    mask = None if token_mask is None else token_mask.contiguous()
+    grad = x.new_empty((n_rows, n_experts)) if want_grad else None
+    counts = x.new_empty(n_experts, dtype=torch.int64)
+    loss = x.new_empty((), dtype=torch.float32)
+    size = _lib.workspace_bytes("fk_moe_balance_workspace_size", logits.device)
+    ws = x.new_empty(size, dtype=torch.uint8)
+    with _lib.on_device(logits):
+        _lib.call("fk_moe_balance", x.data_ptr(), stride, idx.data_ptr(), _lib.ptr(mask), n_rows,
+                  n_experts, idx.shape[1], z_coef, loss_scale, _lib.ptr(grad), counts.data_ptr(),
+                  loss.data_ptr(), ws.data_ptr(), size, _lib.dtype_code(x.dtype),
+                  _lib.stream_of(logits))
+    return loss, counts, grad
+
+
 class _FusedMoEBalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, args):
-        topk_idx, token_mask, z_coef, loss_scale, want_grad = args
-        n_rows, n_experts = logits.shape
-        x, stride = _lib.rows_of(logits, n_experts)
-        idx = topk_idx.to(torch.int64).contiguous()
-        mask = None if token_mask is None else token_mask.contiguous()
-        grad = x.new_empty((n_rows, n_experts)) if want_grad else None
-        counts = x.new_empty(n_experts, dtype=torch.int64)
-        loss = x.new_empty((), dtype=torch.float32)
-        size = _lib.workspace_bytes("fk_moe_balance_workspace_size", logits.device)
-        ws = x.new_empty(size, dtype=torch.uint8)
-        with _lib.on_device(logits):
-            _lib.call("fk_moe_balance", x.data_ptr(), stride, idx.data_ptr(), _lib.ptr(mask),
-                      n_rows, n_experts, idx.shape[1], z_coef, loss_scale, _lib.ptr(grad),
-                      counts.data_ptr(), loss.data_ptr(), ws.data_ptr(), size,
-                      _lib.dtype_code(x.dtype), _lib.stream_of(logits))
-        if want_grad:
-            ctx.grad = grad
-            ctx.loss_scale = loss_scale
-            ctx.set_materialize_grads(False)
-            ctx.mark_non_differentiable(counts)
+        loss, counts, ctx.grad = _balance(logits, *args, True)
+        ctx.loss_scale = args[-1]
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(counts)
         return loss, counts
 
     @staticmethod
@@ -75,6 +78,7 @@ def fused_moe_balance_loss(router_logits: torch.Tensor, topk_idx: torch.Tensor,
         assert token_mask.shape == (n_rows,) and token_mask.dtype == torch.bool
         assert token_mask.device == router_logits.device
     assert 0.0 < loss_scale < float("inf")
-    want_grad = torch.is_grad_enabled() and router_logits.requires_grad
-    return _FusedMoEBalanceLoss.apply(router_logits, (topk_idx, token_mask, float(z_coef),
-                                                      float(loss_scale), want_grad))
+    args = (topk_idx, token_mask, float(z_coef), float(loss_scale))
+    if torch.is_grad_enabled() and router_logits.requires_grad:
+        return _FusedMoEBalanceLoss.apply(router_logits, args)
+    return _balance(router_logits, *args, False)[:2]

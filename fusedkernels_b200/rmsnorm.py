@@ -76,27 +76,32 @@ def _check_add_norm(x, residual, weight):
             "the residual has x's dtype or fp32"
 
 
+def _add_norm(x, residual, w, eps, save):
+    """y, h and (save) rstd."""
+    n_cols = x.shape[-1]
+    n_rows = x.numel() // n_cols
+    x2, xs = _lib.rows_of(x, n_cols)
+    r2, rs = _lib.rows_of(residual, n_cols)
+    y = x.new_empty(x.shape)  # (new_empty: the cheapest of torch's allocating calls)
+    h = residual.new_empty(x.shape)
+    rstd = x.new_empty(n_rows, dtype=torch.float32) if save else None
+    with _lib.on_device(x):
+        _lib.call("fk_add_rmsnorm_fwd", x2.data_ptr(), xs, r2.data_ptr(), rs,
+                  _lib.dtype_code(h.dtype), w.data_ptr(), _lib.dtype_code(w.dtype),
+                  y.data_ptr(), h.data_ptr(), _lib.ptr(rstd), n_rows, n_cols, eps,
+                  _lib.dtype_code(y.dtype), _lib.stream_of(x))
+    return y, h, rstd
+
+
 class _FusedAddRMSNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, weight, eps, save):
-        n_cols = x.shape[-1]
-        n_rows = x.numel() // n_cols
-        x2, xs = _lib.rows_of(x, n_cols)
-        r2, rs = _lib.rows_of(residual, n_cols)
+    def forward(ctx, x, residual, weight, eps):
         w = weight.contiguous()
-        y = x.new_empty(x.shape)  # (new_empty: the cheapest of torch's allocating calls)
-        h = residual.new_empty(x.shape)
-        rstd = x.new_empty(n_rows, dtype=torch.float32) if save else None
-        with _lib.on_device(x):
-            _lib.call("fk_add_rmsnorm_fwd", x2.data_ptr(), xs, r2.data_ptr(), rs,
-                      _lib.dtype_code(h.dtype), w.data_ptr(), _lib.dtype_code(w.dtype),
-                      y.data_ptr(), h.data_ptr(), _lib.ptr(rstd), n_rows, n_cols, eps,
-                      _lib.dtype_code(y.dtype), _lib.stream_of(x))
-        if save:
-            ctx.set_materialize_grads(False)
-            ctx.save_for_backward(h, w, rstd)
-            ctx.x_dtype = x.dtype
-            ctx.weight_shape = weight.shape
+        y, h, rstd = _add_norm(x, residual, w, eps, True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(h, w, rstd)
+        ctx.x_dtype = x.dtype
+        ctx.weight_shape = weight.shape
         return y, h
 
     @staticmethod
@@ -107,10 +112,10 @@ class _FusedAddRMSNormFn(torch.autograd.Function):
         need_x, need_r, need_w = ctx.needs_input_grad[:3]
         if dy is None:  # only the sum was used: its gradient passes through
             if dh is None:
-                return None, None, None, None, None
+                return None, None, None, None
             return (dh.to(ctx.x_dtype) if need_x else None, dh if need_r else None,
                     torch.zeros(ctx.weight_shape, dtype=w.dtype, device=w.device)
-                    if need_w else None, None, None)
+                    if need_w else None, None)
         dy2, dys = _lib.rows_of(dy, n_cols)
         dh2, dhs = (None, 0) if dh is None else _lib.rows_of(dh, n_cols)
         n_rows = h.numel() // n_cols
@@ -126,7 +131,7 @@ class _FusedAddRMSNormFn(torch.autograd.Function):
                       rstd.data_ptr(), dx.data_ptr(), None if dr is dx else dr.data_ptr(),
                       dw.data_ptr(), ws.data_ptr(), size, n_rows, n_cols,
                       _lib.dtype_code(dx.dtype), _lib.stream_of(h))
-        return dx if need_x else None, dr if need_r else None, dw if need_w else None, None, None
+        return dx if need_x else None, dr if need_r else None, dw if need_w else None, None
 
 
 def fused_add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
@@ -139,9 +144,10 @@ def fused_add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Te
     ``FusedRMSNorm``; in the backward pass the gradient that arrives at ``h`` is added in 32
     bits before the one rounding of the inputs' gradient."""
     _check_add_norm(x, residual, weight)
-    save = torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or
-                                        weight.requires_grad)
-    return _FusedAddRMSNormFn.apply(x, residual, weight, float(eps), save)
+    if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or
+                                    weight.requires_grad):
+        return _FusedAddRMSNormFn.apply(x, residual, weight, float(eps))
+    return _add_norm(x, residual, weight.contiguous(), float(eps), False)[:2]
 
 
 def fused_add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None,
