@@ -134,7 +134,9 @@ def check(status: int, name: str) -> None:
 
 def call(name: str, *args) -> None:
     """Call a status-returning entry point and raise RuntimeError on failure."""
-    check(getattr(load(), name)(*args), name)
+    status = getattr(_lib or load(), name)(*args)
+    if status:
+        check(status, name)
 
 
 def dtype_code(dtype: torch.dtype) -> int:

@@ -5,6 +5,10 @@
 //   loss = E/n * sum_t S_t + z/n * sum_t lse_t^2
 //   dloss/dlogits_te = p_te * (E/n * (f_e - S_t) + 2 z/n * lse_t)
 //
+// As the p_te of a token add up to 1, f may be centred: with g_e = f_e - 1/E (formed from the
+// counts, where it is exact) S_t = 1/E + sum_e g_e p_te and f_e - S_t = g_e - sum_j g_j p_tj.  That
+// keeps the gradient's bits where the load is nearly even and f_e and S_t nearly cancel.
+//
 // f depends on the slots alone, so a first small kernel counts them and the second reads
 // every logit once and writes its gradient at once: the logits are not read again in a
 // backward pass.  The counts are integers and the loss is summed in a fixed order, so
@@ -184,7 +188,7 @@ enum Layout { kPacked, kTiled, kSingle };
 
 // What the rows need to know of the counts.
 struct Frame {
-  float f[kMaxExperts];  // share of the slots (NaN after an index out of range)
+  float f[kMaxExperts];  // share of the slots less 1/E (NaN after an index out of range)
   int tot[kCountStride];
   int slots;
   double2 red[kMainWarps];
@@ -214,15 +218,18 @@ __device__ __forceinline__ void read_counts(Frame& fr, const int* part, int n_pa
   if ((tid & 31) == 0) atomicAdd(&fr.slots, mine);
   __syncthreads();
   const int c = tid < n_experts ? fr.tot[tid] : 0;
-  fr.f[tid] = fr.tot[n_experts + 1] ? __int_as_float(0x7fc00000)
-                                    : (float)c / (float)(fr.slots < 1 ? 1 : fr.slots);
+  const double slots = (double)(fr.slots < 1 ? 1 : fr.slots);  // none used: c - slots is 0 too
+  fr.f[tid] = fr.tot[n_experts + 1]
+                  ? __int_as_float(0x7fc00000)
+                  : (float)(((double)c * n_experts - (double)fr.slots) / (slots * n_experts));
   if (blockIdx.x == 0 && tid < n_experts) counts[tid] = c;
   __syncthreads();
 }
 static_assert(kMainThreads == kMaxExperts, "a thread per expert in read_counts");
 
 // Softmax of one token over L lanes with N logits each (-inf past the end): v becomes
-// exp(v - max); returns 1 / sum, the token's S and its logsumexp.
+// exp(v - max); returns 1 / sum (0 where there is none), the token's sum of f p and its
+// logsumexp.
 template <int L, int N>
 __device__ __forceinline__ float token(float (&v)[N], const float (&f)[N], float& s, float& lse) {
   float m = -INFINITY;
@@ -283,17 +290,18 @@ __global__ void __launch_bounds__(kMainThreads, ctas_per_sm<T, LAYOUT, L, PP>())
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % L, n_experts = a.n_experts;
   const int gw = (int)blockIdx.x * kMainWarps + warp, warps = (int)gridDim.x * kMainWarps;
   double sum_s = 0.0, sum_z = 0.0;
-  float ce = 0.f, cz = 0.f;
+  float ce = 0.f, cz = 0.f, even = 0.f;
   auto start = [&] {
     ptx::wait_for_previous_kernel();
     read_counts(fr, part, n_parts, n_experts, a.counts);
     const float n = (float)(fr.tot[n_experts] < 1 ? 1 : fr.tot[n_experts]);
     ce = (float)n_experts * a.loss_scale / n;
     cz = 2.f * a.z_coef * a.loss_scale / n;
+    even = fr.slots < 1 ? 0.f : 1.0f / (float)n_experts;
   };
-  auto add = [&](bool on, float s, float lse) {
-    if (l == 0 && on) {
-      sum_s += (double)s;
+  auto add = [&](bool on, float inv, float s, float lse) {
+    if (l == 0 && on && inv != 0.f) {  // (true for NaN)
+      sum_s += (double)even + (double)s;
       sum_z += (double)lse * (double)lse;
     }
   };
@@ -334,7 +342,7 @@ __global__ void __launch_bounds__(kMainThreads, ctas_per_sm<T, LAYOUT, L, PP>())
           f[i] = fr.f[l + i * L];
         }
         const float inv = token<L, kPer>(v, f, s, lse);
-        add(on, s, lse);
+        add(on, inv, s, lse);
         const float c0 = on ? inv * fmaf(cz, lse, -ce * s) : 0.f, c1 = on ? inv * ce : 0.f;
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
@@ -374,7 +382,7 @@ __global__ void __launch_bounds__(kMainThreads, ctas_per_sm<T, LAYOUT, L, PP>())
       for (int i = 0; i < S::N; ++i) v[i] = cur.get(i);
       S::table(fr.f, l, f);
       const float inv = token<L, S::N>(v, f, s, lse);
-      add(on, s, lse);
+      add(on, inv, s, lse);
       if (grad && row < a.n_rows) {
         const float c0 = on ? inv * fmaf(cz, lse, -ce * s) : 0.f, c1 = on ? inv * ce : 0.f;
 #pragma unroll

@@ -65,6 +65,12 @@ _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _check_add_norm(x, residual, weight):
+    if (x.is_cuda and x.dtype in _FLOATS and weight.dtype in _FLOATS and x.ndim >= 1 and
+            weight.numel() == x.shape[-1] >= 1 and weight.device == x.device and
+            residual is not None and residual.shape == x.shape and
+            residual.device == x.device and
+            (residual.dtype is x.dtype or residual.dtype is torch.float32)):
+        return  # the rule; what is wrong is found out below
     assert x.is_cuda and weight.is_cuda and x.ndim >= 1
     assert x.dtype in _FLOATS and weight.dtype in _FLOATS, "fp32, fp16 or bf16 tensors"
     assert weight.numel() == x.shape[-1] >= 1
@@ -85,11 +91,11 @@ def _add_norm(x, residual, w, eps, save):
     y = x.new_empty(x.shape)  # (new_empty: the cheapest of torch's allocating calls)
     h = residual.new_empty(x.shape)
     rstd = x.new_empty(n_rows, dtype=torch.float32) if save else None
+    code = _lib._DTYPE_CODES
     with _lib.on_device(x):
-        _lib.call("fk_add_rmsnorm_fwd", x2.data_ptr(), xs, r2.data_ptr(), rs,
-                  _lib.dtype_code(h.dtype), w.data_ptr(), _lib.dtype_code(w.dtype),
-                  y.data_ptr(), h.data_ptr(), _lib.ptr(rstd), n_rows, n_cols, eps,
-                  _lib.dtype_code(y.dtype), _lib.stream_of(x))
+        _lib.call("fk_add_rmsnorm_fwd", x2.data_ptr(), xs, r2.data_ptr(), rs, code[h.dtype],
+                  w.data_ptr(), code[w.dtype], y.data_ptr(), h.data_ptr(), _lib.ptr(rstd), n_rows,
+                  n_cols, eps, code[y.dtype], _lib.stream_of(x))
     return y, h, rstd
 
 
@@ -125,12 +131,12 @@ class _FusedAddRMSNormFn(torch.autograd.Function):
         size = _lib.workspace_bytes("fk_add_rmsnorm_bwd_workspace_size", h.device, n_rows,
                                     n_cols)
         ws = h.new_empty(size, dtype=torch.uint8)
+        code = _lib._DTYPE_CODES
         with _lib.on_device(h):
             _lib.call("fk_add_rmsnorm_bwd", dy2.data_ptr(), dys, _lib.ptr(dh2), dhs, h.data_ptr(),
-                      _lib.dtype_code(h.dtype), w.data_ptr(), _lib.dtype_code(w.dtype),
-                      rstd.data_ptr(), dx.data_ptr(), None if dr is dx else dr.data_ptr(),
-                      dw.data_ptr(), ws.data_ptr(), size, n_rows, n_cols,
-                      _lib.dtype_code(dx.dtype), _lib.stream_of(h))
+                      code[h.dtype], w.data_ptr(), code[w.dtype], rstd.data_ptr(), dx.data_ptr(),
+                      None if dr is dx else dr.data_ptr(), dw.data_ptr(), ws.data_ptr(), size,
+                      n_rows, n_cols, code[dx.dtype], _lib.stream_of(h))
         return dx if need_x else None, dr if need_r else None, dw if need_w else None, None
 
 

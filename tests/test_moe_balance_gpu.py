@@ -104,6 +104,26 @@ def test_masked_away_and_unused_slots():
     assert_within(xg.grad, wgrad, 2 * gb + half_step(FP) * wgrad.abs())
 
 
+@pytest.mark.parametrize("e", [8, 7, 100])
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_even_load(e, dtype):
+    """Every expert chosen by every token: f is 1/E, the loss 1 and the gradient nothing but 0.
+    With one expert spared per token the gradient is all cancellation; it keeps its bits: 64
+    roundings of p (f - 1/E) terms, not of p f ones."""
+    logits, idx, _ = inputs(300, e, e, dtype, seed=e)
+    loss, _, grad = check(logits, idx, None)
+    assert loss == 1.0 and torch.count_nonzero(grad) == 0
+    logits = logits.float()
+    idx = logits.topk(e - 1, dim=1).indices
+    _, _, grad = check(logits, idx, None)
+    _, counts, want, _, _ = balance(logits, idx, None, 0.0)
+    g = counts.double() / idx.numel() - 1 / e
+    p = torch.softmax(logits.double(), 1)
+    size = e / 300 * p * (g.abs() + (p * g.abs()).sum(1, keepdim=True))
+    far = float(logits.abs().max())
+    assert_within(grad, want, (64 + 4 * far) * 2.0 ** -24 * size)
+
+
 def test_infinite_logits():
     logits, idx, _ = inputs(20, 12, 2, FP, seed=6)
     logits[:, 3] = -float("inf")  # an expert that is switched off
