@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(256) add_rmsnorm_bwd_lanes(BwdArgs a) {
 // Longer rows: the CTA takes a row.  Rows of dy, h and dh arrive in a ring of shared-memory
 // stages by cp.async.bulk; a stage is refilled as soon as all threads have its chunks in
 // registers, which the reduction's barrier tells.  Bound by HBM: 86 us at 16384 x 4096 bf16 (6.3
-// TB/s), 4 us more for dw.  Stages: 3 where they take 72 KB (three CTAs an SM), else 2.
+// TB/s), 4 us more for dw.  Stages: 3 where they take 72 KB (three CTAs an SM), else 2, or 1.
 constexpr int kBwdMaxStages = 4;
 template <typename T, typename R, int THREADS, int CPT>
 __global__ void __launch_bounds__(THREADS) add_rmsnorm_bwd_ring(BwdArgs a, int stages) {
@@ -605,8 +605,10 @@ int launch_bwd_ring(const BwdArgs& a, int* grid, cudaStream_t st) {
   constexpr auto kern = add_rmsnorm_bwd_ring<T, R, THREADS, CPT>;
   allow_shared_memory<kern>(1024);
   const int stage = a.cols * ((int)sizeof(T) + (a.dh ? 2 : 1) * (int)sizeof(R));
+  constexpr int kMost = 224 * 1024;  // of a CTA
+  if (stage > kMost) return -1;
   int stages = 72 * 1024 / stage;
-  stages = stages < 2 ? 2 : stages > 3 ? 3 : stages;
+  stages = stages >= 3 ? 3 : 2 * stage <= kMost ? 2 : 1;
   const int smem = stages * stage;
   const int most = num_sms() * resident_ctas<kern>(THREADS, smem);
   *grid = a.rows < most ? a.rows : most;
@@ -629,6 +631,7 @@ int bwd_chunked(const BwdArgs& a, int* grid, cudaStream_t st) {
   if (chunks <= 256) return launch_bwd_ring<T, R, 128, 2>(a, grid, st);
   if (chunks <= 512) return launch_bwd_ring<T, R, 256, 2>(a, grid, st);
   if (chunks <= 1024) return launch_bwd_ring<T, R, 512, 2>(a, grid, st);
+  if (chunks <= 2048) return launch_bwd_ring<T, R, 1024, 2>(a, grid, st);
   return -1;
 }
 
