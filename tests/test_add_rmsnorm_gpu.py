@@ -335,3 +335,54 @@ def test_quant_graph_replay():
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+# In fp32 the forward's y is the very y that is quantised: its row sum has the same terms in the
+# same order.  So scales and bytes have to be those of the 32-bit divisions, bit for bit.
+def divided(y, block):
+    b = block or y.shape[-1]
+    parts = y.split(b, dim=-1)
+    scales = torch.stack([p.abs().amax(-1) for p in parts], -1).div(448).clamp(min=2.0 ** -126)
+    q = torch.cat([p / scales[..., i:i + 1] for i, p in enumerate(parts)], -1)
+    return q.clamp(-448, 448).to(torch.float8_e4m3fn), scales
+
+
+def assert_divided(got, y, block):
+    q, scales = divided(y.cpu(), block)
+    assert torch.equal(got[1].cpu(), scales)
+    assert torch.equal(got[0].cpu().view(torch.uint8), q.view(torch.uint8))
+
+
+@pytest.mark.parametrize("block", [None, 128])
+@pytest.mark.parametrize("shape", [(700, 64), (64, 4096), (2048, 2048), (400, 1111), (9, 8192),
+                                   (3, 16400)], ids=str)
+def test_quant_is_a_division(shape, block):
+    """Short rows to the longest, whole packets, single elements and element loops."""
+    x, r, w, _, _ = inputs(shape, FP, FP, FP, seed=24)
+    for row, size in enumerate((1e-26, 1e-30, 1e-34)[:shape[0]]):  # rows far below eps: tiny scales
+        x[row] *= size
+        r[row] *= size
+    w[0], w[1], w[2] = 0.0, 1e30, 1e33  # zeros of both signs; large scales
+    xg, rg, wg = x.cuda(), r.cuda(), w.cuda()
+    with torch.no_grad():
+        y, _ = fk.fused_add_rms_norm(xg, rg, wg, EPS)
+        assert_divided(fk.fused_add_rms_norm_quant(xg, rg, wg, EPS, block=block), y, block)
+        wg[:3] = 1.0
+        y, _ = fk.fused_add_rms_norm(xg, rg, wg, EPS)
+        assert_divided(fk.fused_add_rms_norm_quant(xg, rg, wg, EPS, block=block), y, block)
+
+
+@pytest.mark.parametrize("block", [None, 128])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("cols", [4096, 1111])
+def test_quant_is_a_division_in_16_bits(cols, dtype, block):
+    """Rows of +1 and -1: the sum of squares is exact in any order, so the 32-bit y of the same
+    values in fp32 is known beside a 16-bit x."""
+    G = gen(25)
+    x = (torch.randint(0, 2, (500, cols), generator=G) * 2 - 1).to(dtype).cuda()
+    w = (1 + 0.5 * torch.randn(cols, generator=G)).cuda()
+    w[5] = 0.0
+    with torch.no_grad():
+        y, _ = fk.fused_add_rms_norm(x.float(), torch.zeros(500, cols, device="cuda"), w, EPS)
+        for r in (None, torch.zeros_like(x), torch.zeros(500, cols, device="cuda")):
+            assert_divided(fk.fused_add_rms_norm_quant(x, r, w, EPS, block=block), y, block)
