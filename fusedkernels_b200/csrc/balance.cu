@@ -351,7 +351,8 @@ __global__ void __launch_bounds__(kMainThreads, ctas_per_sm<T, LAYOUT, L, PP>())
       __syncwarp();
       if (grad) {
         T* dst = grad + (int64_t)t * kRows * n_experts;
-        const int left = (a.n_rows - t * kRows) * n_experts;  // elements
+        const int rows = a.n_rows - t * kRows;
+        const int left = (rows < kRows ? rows : kRows) * n_experts;  // elements of the tile
         for (int u = lane; u < n_experts; u += 32) {
           if ((u + 1) * kRows <= left)
             __stcs(reinterpret_cast<uint4*>(dst) + u, reinterpret_cast<const uint4*>(tile)[u]);
