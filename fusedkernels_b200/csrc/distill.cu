@@ -16,6 +16,8 @@
 #include "exp.cuh"
 #include "ptx.cuh"
 
+#include <type_traits>
+
 namespace fk {
 namespace {
 
@@ -535,6 +537,11 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
     f = a.q2 ? b2 : b;
     f1 = b2 * (a.p4 ? b2 : b);
   };
+  auto powers_of_pair = [&](float2 b, float2& f, float2& f1) {
+    const float2 b2 = __fmul2_rn(b, b);
+    f = a.q2 ? b2 : b;
+    f1 = __fmul2_rn(b2, a.p4 ? b2 : b);
+  };
   const bool same_slice = lstride % VN == 0;  // every row has the first row's offset
   const bool lists = warp * 32 < a.list;      // this warp has listed elements to handle
   bool ok = true;
@@ -624,13 +631,14 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
       my_m = fmaxf(fmaxf(f.x, f.y), xs);
     }
     const float base = my_m == -INFINITY ? 0.f : my_m;
-    const float nb_t = -base * ct_row, nb_1 = -base * kLog2e;
+    // The maximum goes off first: folded into the exponent as the constant -max log2(e) / T it would
+    // leave that product's rounding in every term, and overflow at a mask of the type's lowest value.
     auto exp_one = [&](float x, float& f, float& f1) {
+      const float d = x - base;
       if constexpr (sizeof(T) == 2) {
-        f = ex2f(fmaf(x, ct_row, nb_t));
-        if constexpr (M == kTwo) f1 = ex2f(fmaf(x, kLog2e, nb_1));
+        f = ex2f(d * ct_row);
+        if constexpr (M == kTwo) f1 = ex2f(d * kLog2e);
       } else {
-        const float d = x - base;
         f = exp2_of(d * inv_b);
         if constexpr (M == kTwo) f1 = exp2_of(d);
       }
@@ -649,12 +657,12 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
         const float2 x = p[u].p[k].f();
         float2 f, f1 = make_float2(0.f, 0.f);
         if constexpr (sizeof(T) == 2 && M != kTwo) {
-          const float2 t = __ffma2_rn(x, make_float2(ct_row, ct_row), make_float2(nb_t, nb_t));
+          const float2 t = __fmul2_rn(__fadd2_rn(x, make_float2(-base, -base)),
+                                      make_float2(ct_row, ct_row));
           f = make_float2(ex2f(t.x), ex2f(t.y));
           if constexpr (M == kPowers) {
             float2 g;
-            powers(f.x, g.x, f1.x);
-            powers(f.y, g.y, f1.y);
+            powers_of_pair(f, g, f1);
             z = __fadd2_rn(z, g);
             z1 = __fadd2_rn(z1, f1);
           } else {
@@ -722,7 +730,7 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
         if (xs_at >= 0) dst[xs_at] = Elt<T>::from_f(fill);
       } else {
         // 16 bits: the factor k / z goes into the exponent.
-        const float ot = fmaf(-st.m, ct_row, __log2f(kt)), o1 = fmaf(-st.m, kLog2e, __log2f(k1));
+        const float ot = __log2f(kt), o1 = __log2f(k1);
         // wt exp(d / T) and, where one exponential gives both, + w1 exp(d).
         auto both = [&](float b, float wt, float w1) {
           if constexpr (M == kPowers) {
@@ -733,17 +741,16 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
           return b * (M == kSquare ? fmaf(b, w1, wt) : wt);
         };
         auto dense = [&](float x) {
+          const float d = x - st.m;
           float g;
           if constexpr (sizeof(T) == 2) {
             if constexpr (M == kSquare || M == kPowers) {
-              const float b = ex2f(fmaf(x, ct_row, -st.m * ct_row));
-              g = both(b, kt, k1);
+              g = both(ex2f(d * ct_row), kt, k1);
             } else {
-              g = ex2f(fmaf(x, ct_row, ot));
-              if constexpr (M == kTwo) g += ex2f(fmaf(x, kLog2e, o1));
+              g = ex2f(fmaf(d, ct_row, ot));
+              if constexpr (M == kTwo) g += ex2f(fmaf(d, kLog2e, o1));
             }
           } else {
-            const float d = x - st.m;
             g = both(exp2_of(d * inv_b), kt, k1);
             if constexpr (M == kTwo) g = fmaf(exp2_of(d), k1, g);
           }
@@ -769,9 +776,28 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
               o.p[k].set(g);
             } else {
               const float2 x = p[u].p[k].f();
-              if constexpr (sizeof(T) == 2 && M == kOne) {
-                const float2 t = __ffma2_rn(x, make_float2(ct_row, ct_row), make_float2(ot, ot));
-                o.p[k].set(make_float2(ex2f(t.x), ex2f(t.y)));
+              if constexpr (sizeof(T) == 2 && M != kTwo) {
+                const float2 c = make_float2(ct_row, ct_row);
+                if constexpr (M == kOne) {
+                  // (fp16: the maximum as a pair, beside the other two, spills: 249 against 237 us
+                  // at 8192 x 32000; bf16: single 788, as a pair 783 at 8192 x 128256.)
+                  float2 d = make_float2(x.x - st.m, x.y - st.m);
+                  if (std::is_same<T, __nv_bfloat16>::value)
+                    d = __fadd2_rn(x, make_float2(-st.m, -st.m));
+                  const float2 t = __ffma2_rn(d, c, make_float2(ot, ot));
+                  o.p[k].set(make_float2(ex2f(t.x), ex2f(t.y)));
+                } else {
+                  const float2 t = __fmul2_rn(__fadd2_rn(x, make_float2(-st.m, -st.m)), c);
+                  const float2 b = make_float2(ex2f(t.x), ex2f(t.y));
+                  const float2 wt = make_float2(kt, kt), w1 = make_float2(k1, k1);
+                  if constexpr (M == kPowers) {
+                    float2 f, f1;
+                    powers_of_pair(b, f, f1);
+                    o.p[k].set(__ffma2_rn(f1, w1, __fmul2_rn(f, wt)));
+                  } else {
+                    o.p[k].set(__fmul2_rn(b, __ffma2_rn(b, w1, wt)));
+                  }
+                }
               } else {
                 o.p[k].set(make_float2(dense(x.x), dense(x.y)));
               }
