@@ -11,6 +11,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libfkb200.so"
 
@@ -228,6 +229,19 @@ def rows_of(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int]:
     if cols > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < cols:
         return t.contiguous(), cols
     return t, max(t.stride(0), cols)  # a tensor of one row may report any stride
+
+
+def wants_derivative(*tensors) -> bool:
+    """Whether autograd has to see an operator's call: some input requires a gradient, or carries
+    a tangent of forward mode (which an autograd.Function without a jvp refuses)."""
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors) or \
+        has_tangent(*tensors)
+
+
+def has_tangent(*tensors) -> bool:
+    if forward_ad._current_level < 0:  # outside every dual_level: none can
+        return False
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _NoSecondDerivative(torch.autograd.Function):

@@ -94,7 +94,8 @@ def fused_distillation_loss(logits: torch.Tensor, teacher_idx: torch.Tensor,
         f"the teacher has one row of 1..{MAX_SLOTS} slots for each row of logits"
     assert teacher_idx.dtype in (torch.int64, torch.int32)
     assert teacher_idx.device == logits.device and teacher_logits.device == logits.device
-    assert not teacher_logits.requires_grad, "the teacher gets no gradient: detach its logits"
+    assert not teacher_logits.requires_grad and not _lib.has_tangent(teacher_logits), \
+        "the teacher gets no gradient: detach its logits"
     if targets is not None:
         assert targets.shape == (n_rows,) and targets.device == logits.device
         assert not targets.is_floating_point()
@@ -102,7 +103,7 @@ def fused_distillation_loss(logits: torch.Tensor, teacher_idx: torch.Tensor,
     assert 0.0 < loss_scale < float("inf")
     args = (teacher_idx, teacher_logits, targets, float(temperature), float(hard_weight),
             int(ignore_index), inplace_grad, float(loss_scale))
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _lib.wants_derivative(logits):
         return _FusedDistillation.apply(logits, args)
     return _distill(logits, *args, False)[0]
 

@@ -79,6 +79,6 @@ def fused_moe_balance_loss(router_logits: torch.Tensor, topk_idx: torch.Tensor,
         assert token_mask.device == router_logits.device
     assert 0.0 < loss_scale < float("inf")
     args = (topk_idx, token_mask, float(z_coef), float(loss_scale))
-    if torch.is_grad_enabled() and router_logits.requires_grad:
+    if _lib.wants_derivative(router_logits):
         return _FusedMoEBalanceLoss.apply(router_logits, args)
     return _balance(router_logits, *args, False)[:2]

@@ -150,8 +150,7 @@ def fused_add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Te
     ``FusedRMSNorm``; in the backward pass the gradient that arrives at ``h`` is added in 32
     bits before the one rounding of the inputs' gradient."""
     _check_add_norm(x, residual, weight)
-    if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or
-                                    weight.requires_grad):
+    if _lib.wants_derivative(x, residual, weight):
         return _FusedAddRMSNormFn.apply(x, residual, weight, float(eps))
     return _add_norm(x, residual, weight.contiguous(), float(eps), False)[:2]
 
@@ -169,9 +168,7 @@ def fused_add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None,
     8-bit side of a product: it has no gradient, and asserts that none is asked for."""
     _check_add_norm(x, residual, weight)
     assert block in (None, 128), "block is None (a scale per row) or 128"
-    assert not (torch.is_grad_enabled() and
-                (x.requires_grad or weight.requires_grad or
-                 (residual is not None and residual.requires_grad))), \
+    assert not _lib.wants_derivative(x, weight, *(() if residual is None else (residual,))), \
         "fused_add_rms_norm_quant has no gradient: call it under torch.no_grad()"
     n_cols = x.shape[-1]
     n_rows = x.numel() // n_cols
