@@ -563,10 +563,11 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_bwd_ring(BwdArgs a, int s
         }
       }
     }
+    // (A thread whose wait ran out poisons the row for all of them, and its part of dw below.)
+    if (!ok) dot = __int_as_float(0x7fc00000);
     dot = row_reduce<THREADS, false>(dot, red[parity]);  // its barrier frees the stage
-    if (tid == 0) issue(row + stages * step, q);
-    // (A wait that ran out poisons the row.)
-    const float c2 = ok ? s * s * s * (dot * inv_cols) : __int_as_float(0x7fc00000);
+    if (tid == 0 && ok) issue(row + stages * step, q);
+    const float c2 = s * s * s * (dot * inv_cols);
 #pragma unroll
     for (int u = 0; u < CPT; ++u) {
       const int c = tid + u * THREADS;
@@ -590,6 +591,11 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_bwd_ring(BwdArgs a, int s
       for (int k = 0; k < VN; k += 4)
         *reinterpret_cast<float4*>(prow + c * VN + k) =
             make_float4(acc[u][k], acc[u][k + 1], acc[u][k + 2], acc[u][k + 3]);
+  }
+  if (!ok) {  // what came late or not at all is in the sums, and may still be on its way
+    for (int c = tid; c < chunks; c += THREADS)
+      for (int k = 0; k < VN; ++k) prow[c * VN + k] = __int_as_float(0x7fc00000);
+    for (int i = 0; i < 2 * stages; ++i) ptx::mbar_wait(&full[i >> 1], (uint32_t)(i & 1), kPolls);
   }
 }
 
