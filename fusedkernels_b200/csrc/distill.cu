@@ -689,10 +689,12 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
           if constexpr (M == kTwo) e1[u][k] = f1;
         }
       }
+    // (A thread whose wait ran out poisons the row's sums for all of them.)
+    if (!ok) z.x = __int_as_float(0x7fc00000);
     Stat st = join<T, M, 32>(Stat{my_m, z.x + z.y, M != kOne ? z1.x + z1.y : 0.f}, inv_t);
     if (lane == 0) wred[warp] = st;
     __syncthreads();  // the stage has been read by all
-    if (loader) issue(row + stages * step, q);
+    if (loader && ok) issue(row + stages * step, q);
     if (C == 1 || warp == 0) st = join<T, M, kWarps>(wred[lane & (kWarps - 1)], inv_t);
     if (C > 1) {
       if (warp == 0) {
@@ -711,7 +713,7 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
     } else {
       read_ahead(row + step);
     }
-    if (!ok) st.z = st.z1 = __int_as_float(0x7fc00000);  // a wait ran out: the row is poisoned
+    if (!ok) st.z = st.z1 = __int_as_float(0x7fc00000);  // (or the wait for the other CTAs)
     const float hw = (row_state & kHard) ? a.hard_weight : 0.f;
     const float sw = (row_state & kSoft) ? 1.f - a.hard_weight : 0.f;
     const float ct = sw * a.temperature * a.loss_scale * inv_n, c1 = hw * a.loss_scale * inv_n;
@@ -851,6 +853,10 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
     src += step * lstride;
     dst += step * gstride;
     if (!same_slice) sl = slice_of(src);
+  }
+  if (!ok) {  // the loss is poisoned too; what may still be on its way is waited for once more
+    total = __longlong_as_double(0x7ff8000000000000ll);
+    for (int i = 0; i < 2 * stages; ++i) ptx::mbar_wait(&full[i >> 1], (uint32_t)(i & 1), kPolls);
   }
   if (C > 1) ptx::cluster_sync();  // nobody's shared memory is written after its CTA is gone
   finish_loss(a, 1.0f / inv_n, total);
