@@ -285,7 +285,7 @@ __device__ __forceinline__ double block_total(double s) {
 
 // Every thread brings its part of the loss of the CTA's rows; the CTA that ends last adds the
 // CTAs' sums up in a fixed order (at most 16 per SM).
-__device__ __forceinline__ void finish_loss(const RowArgs& a, float n, double mine) {
+__device__ __forceinline__ void finish_loss(const RowArgs& a, double mine) {
   __shared__ bool last;
   mine = block_total(mine);
   if (threadIdx.x == 0) {
@@ -302,6 +302,7 @@ __device__ __forceinline__ void finish_loss(const RowArgs& a, float n, double mi
   int bad = 0;
   for (int i = threadIdx.x; i < a.teacher_ctas; i += blockDim.x) bad |= a.valid[i].y;
   bad = __syncthreads_or(bad);
+  const float n = count_valid(a);
   if (threadIdx.x == 0) {
     *a.loss = (float)(s / (double)n);
     *a.err = bad != 0;
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(kGenericThreads) distill_rows_generic(
     }
     __syncthreads();  // picked is the next row's from here
   }
-  finish_loss(a, n, total);
+  finish_loss(a, total);
 }
 
 // ------------------------------------------------------------------ rows, 16-byte packets
@@ -859,7 +860,7 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
     for (int i = 0; i < 2 * stages; ++i) ptx::mbar_wait(&full[i >> 1], (uint32_t)(i & 1), kPolls);
   }
   if (C > 1) ptx::cluster_sync();  // nobody's shared memory is written after its CTA is gone
-  finish_loss(a, 1.0f / inv_n, total);
+  finish_loss(a, total);
 }
 
 template <typename T, Mode M, bool KEEP, int THREADS, int KP, int MIN_CTAS>

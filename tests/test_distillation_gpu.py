@@ -308,3 +308,23 @@ def test_graph_replay_beside_another_stream():
     for (logits, idx, top, targets), (_, loss, grad, _) in zip(sets, graphs):
         eager = check(logits, idx, top, targets)
         assert torch.equal(eager[0], loss) and torch.equal(eager[1], grad)
+
+
+@pytest.mark.parametrize("v", [600, 601])
+def test_mean_of_equal_rows(v):
+    """n times the same row: the sum in 64 bits is n times that row's loss, so the mean is the one
+    row's loss, bit for bit (601 with a gradient at another offset takes the element loops)."""
+    logits, idx, top, targets = inputs(1, v, 6, FP, seed=16, ragged=False)
+    targets[:] = 5
+
+    def loss(n):
+        x = logits.expand(n, v).contiguous().cuda()
+        if v == 601:
+            x = torch.nn.functional.pad(x, (1, 2))[:, 1:602]
+        x.requires_grad_(True)
+        return fk.fused_distillation_loss(x, idx.expand(n, -1).cuda(), top.expand(n, -1).cuda(),
+                                          targets.expand(n).cuda()).detach()
+
+    one = loss(1)
+    for n in (3, 7, 13, 14, 15, 26, 41, 47, 55):  # 1 / (1 / n) is not n in 32 bits for most
+        assert torch.equal(loss(n), one), n
