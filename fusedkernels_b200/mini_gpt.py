@@ -128,8 +128,9 @@ class MiniGPT(nn.Module):
         return self.lm_head(x).reshape(B * T, -1)
 
     def balance_loss(self):
-        """Sum of the MoE blocks' balance losses of the last forward (0 where none asks)."""
-        losses = [b.mlp.balance_loss for b in self.blocks]
+        """Sum of the MoE blocks' balance losses of the last forward (0 where none asks, and for a
+        model without MoE blocks)."""
+        losses = [getattr(b.mlp, "balance_loss", None) for b in self.blocks]
         return sum(x for x in losses if x is not None)
 
     @torch.no_grad()
