@@ -65,20 +65,13 @@ _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _check_add_norm(x, residual, weight):
-    if (x.is_cuda and x.dtype in _FLOATS and weight.dtype in _FLOATS and x.ndim >= 1 and
-            weight.numel() == x.shape[-1] >= 1 and weight.device == x.device and
-            residual is not None and residual.shape == x.shape and
-            residual.device == x.device and
-            (residual.dtype is x.dtype or residual.dtype is torch.float32)):
-        return  # the rule; what is wrong is found out below
-    assert x.is_cuda and weight.is_cuda and x.ndim >= 1
+    assert x.is_cuda and x.ndim >= 1 and weight.device == x.device
     assert x.dtype in _FLOATS and weight.dtype in _FLOATS, "fp32, fp16 or bf16 tensors"
     assert weight.numel() == x.shape[-1] >= 1
-    assert weight.device == x.device
     if residual is not None:
         assert residual.shape == x.shape, "residual and x have one shape (nothing is broadcast)"
         assert residual.device == x.device
-        assert residual.dtype == x.dtype or residual.dtype == torch.float32, \
+        assert residual.dtype is x.dtype or residual.dtype is torch.float32, \
             "the residual has x's dtype or fp32"
 
 
@@ -149,6 +142,7 @@ def fused_add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Te
     The norm is that of the rounded ``h``, so the result is that of the addition followed by
     ``FusedRMSNorm``; in the backward pass the gradient that arrives at ``h`` is added in 32
     bits before the one rounding of the inputs' gradient."""
+    assert residual is not None, "without a residual there is nothing to add: call FusedRMSNorm"
     _check_add_norm(x, residual, weight)
     if _lib.wants_derivative(x, residual, weight):
         return _FusedAddRMSNormFn.apply(x, residual, weight, float(eps))

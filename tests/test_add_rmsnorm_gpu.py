@@ -386,3 +386,10 @@ def test_quant_is_a_division_in_16_bits(cols, dtype, block):
         y, _ = fk.fused_add_rms_norm(x.float(), torch.zeros(500, cols, device="cuda"), w, EPS)
         for r in (None, torch.zeros_like(x), torch.zeros(500, cols, device="cuda")):
             assert_divided(fk.fused_add_rms_norm_quant(x, r, w, EPS, block=block), y, block)
+
+
+def test_no_residual_is_refused():
+    """(The module and the 8-bit form take None.)"""
+    x, w = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    with pytest.raises(AssertionError, match="residual"):
+        fk.fused_add_rms_norm(x, None, w)
