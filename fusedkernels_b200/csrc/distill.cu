@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kGenericThreads) distill_rows_generic(
       for (int j = threadIdx.x; j < a.list; j += blockDim.x) {
         const int c = ids[j];
         if (c >= 0)
-          dst[c] = Elt<T>::from_f(dense(picked[j]) - ct * probs[j] -
+          dst[c] = Elt<T>::from_f(dense(picked[j]) - (sw > 0.f ? ct * probs[j] : 0.f) -
                                   ((state & kHard) && j == a.list - 1 ? c1 : 0.f));
       }
     }
@@ -813,8 +813,8 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
       }
     }
     __syncthreads();  // the listed places are written over the dense values
-    // The listed elements of this CTA: their part of the loss, and their gradient.  A part of
-    // the loss whose weight is 0 is left out, even where it is infinite.
+    // The listed elements of this CTA: their part of the loss, and their gradient.  A part whose
+    // weight is 0 is left out, even where it is infinite or NaN.
     float l = 0.f;
     auto listed = [&](int j, int c, float x, float pj) {
       const float d = x - st.m;
@@ -822,7 +822,7 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
       if (sw > 0.f && pj != 0.f) l -= sw * a.temperature * pj * d;
       if (hw > 0.f && label) l -= hw * d;
       if (grad) {
-        float g = kt * exp_of<T>(d * inv_t) - ct * pj;
+        float g = kt * exp_of<T>(d * inv_t) - (sw > 0.f ? ct * pj : 0.f);
         if constexpr (M != kOne) g = fmaf(k1, exp_of<T>(d), g);
         if (label) g -= c1;
         dst[c] = Elt<T>::from_f(g);

@@ -77,6 +77,7 @@ def fused_distillation_loss(logits: torch.Tensor, teacher_idx: torch.Tensor,
     targets: [N] hard labels.  With them the counted rows are those whose target is not
     ignore_index, and hard_weight mixes the two parts; without them the counted rows are those
     that hold a teacher, and the loss is the soft part alone (hard_weight is not used).
+    With hard_weight 1 (or 0) the soft (hard) part is left out, whatever the teacher's logits hold.
     inplace_grad=True writes the gradient over the logits buffer, as in fused_cross_entropy;
     where no gradient is wanted the logits are left as they are.
     loss_scale: the factor that the backward pass will be started with (a GradScaler's scale).

@@ -328,3 +328,20 @@ def test_mean_of_equal_rows(v):
     one = loss(1)
     for n in (3, 7, 13, 14, 15, 26, 41, 47, 55):  # 1 / (1 / n) is not n in 32 bits for most
         assert torch.equal(loss(n), one), n
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("v", [1000, 1003, 4096])
+def test_hard_weight_one_leaves_the_teacher_out(v, dtype):
+    """Even where its logits are NaN or infinite."""
+    logits, idx, top, targets = inputs(8, v, 6, dtype, seed=17, ragged=False)
+    targets[:] = idx[:, 1]
+    top[0, 1], top[1, 1], top[2, 3] = float("nan"), float("inf"), float("inf")
+    top[4] = float("nan")
+    for temperature in (1.0, 2.0):
+        _, grad = check(logits, idx, top, targets, temperature, hard_weight=1.0)
+        assert torch.isfinite(grad).all()
+    wide = torch.zeros(8, v + 13, dtype=dtype, device="cuda")
+    wide[:, 3:v + 3] = logits.cuda()  # the element loops
+    check(logits, idx, top, targets, 2.0, hard_weight=1.0,
+          xg=wide[:, 3:v + 3].detach().requires_grad_(True))
