@@ -371,6 +371,10 @@ int rows_single(const FwdArgs& a, cudaStream_t st) {
   return -1;
 }
 
+// mean(w dy h) s^3, s times three: s^3 by itself leaves the normal range where a row's size is
+// beyond 1e12, while the product is of the size of dy / h^2.
+__device__ __forceinline__ float times_cube(float mean, float s) { return mean * s * s * s; }
+
 // ------------------------------------------------------------------ backward, chunks ----
 // Persistent CTAs, so that dw is summed in registers: a thread has the same columns in every
 // row it meets.  Each CTA leaves one partial row of dw; a second kernel adds those up.
@@ -463,7 +467,7 @@ __global__ void __launch_bounds__(256) add_rmsnorm_bwd_lanes(BwdArgs a) {
           acc[u][k] = fmaf(d * hv, s, acc[u][k]);
         }
     dot = row_reduce<TPR, false>(dot, nullptr);
-    const float c2 = s * s * s * (dot * inv_cols);
+    const float c2 = times_cube(dot * inv_cols, s);
 #pragma unroll
     for (int u = 0; u < CPT; ++u) {
       const int c = t + u * TPR;
@@ -567,7 +571,7 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_bwd_ring(BwdArgs a, int s
     if (!ok) dot = __int_as_float(0x7fc00000);
     dot = row_reduce<THREADS, false>(dot, red[parity]);  // its barrier frees the stage
     if (tid == 0 && ok) issue(row + stages * step, q);
-    const float c2 = s * s * s * (dot * inv_cols);
+    const float c2 = times_cube(dot * inv_cols, s);
 #pragma unroll
     for (int u = 0; u < CPT; ++u) {
       const int c = tid + u * THREADS;
@@ -718,7 +722,7 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_bwd_columns(BwdArgs a) {
     }
     load(row + step);
     dot = row_reduce<THREADS, false>(dot, red[parity]);
-    const float c2 = s * s * s * (dot * inv_cols);
+    const float c2 = times_cube(dot * inv_cols, s);
     T* px = static_cast<T*>(a.dx) + (int64_t)row * a.cols;
     R* pr = static_cast<R*>(a.dr) + (int64_t)row * a.cols;
 #pragma unroll
@@ -798,7 +802,7 @@ __global__ void __launch_bounds__(256) add_rmsnorm_bwd_generic(
       dot = fmaf(load_wd(w, wd, c) * d, hv, dot);
       prow[c] = fmaf(d * hv, s, prow[c]);  // each column is one thread's
     }
-    const float c2 = s * s * s * (block_sum(dot, red) / (float)cols);
+    const float c2 = times_cube(block_sum(dot, red) / (float)cols, s);
     for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) {
       const float d = Elt<T>::to_f(dy[row * dys + c]), hv = Elt<R>::to_f(h[row * cols + c]);
       float g = s * (load_wd(w, wd, c) * d) - hv * c2;

@@ -393,3 +393,13 @@ def test_no_residual_is_refused():
     x, w = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
     with pytest.raises(AssertionError, match="residual"):
         fk.fused_add_rms_norm(x, None, w)
+
+
+@pytest.mark.parametrize("types", [(FP, FP), (BF, BF), (BF, FP)], ids=str)
+@pytest.mark.parametrize("cols", [64, 1000, 1111, 4096, 40000])
+@pytest.mark.parametrize("size", [1e-12, 1e10, 1e14, 1e16])
+def test_gradient_of_rows_of_any_size(size, cols, types):
+    """s^3 leaves the normal range of fp32 at 1e13 and more, the gradient does not."""
+    x, r, w, dy, _ = inputs((6, cols), *types, FP, seed=31)
+    x, r = (x.double() * size).to(types[0]), (r.double() * size).to(types[1])
+    check(x, r, w, dy, None, *leaves(x, r, w))
