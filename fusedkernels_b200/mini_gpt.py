@@ -115,6 +115,9 @@ class MiniGPT(nn.Module):
     def logits(self, idx):
         """Logits [B * T, vocab_size] of a batch of tokens."""
         B, T = idx.shape
+        if self.n_experts:
+            for blk in self.blocks:  # a later block's would keep the graph of the earlier ones
+                blk.mlp.balance_loss = None
         x = self.tok_emb(idx) + self.pos_emb(torch.arange(T, device=idx.device))[None]
         if self.fused_residual:
             residual = None

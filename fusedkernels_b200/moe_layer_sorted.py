@@ -29,6 +29,8 @@ Every GEMM runs on the tcgen05 tensor cores in the layer's dtype: bf16 and fp16 
 3xTF32 split (each fp32 operand becomes a tf32 hi part plus a residual, and the kernel
 sums hi*hi + hi*lo + lo*hi in fp32), which keeps fp32-class accuracy.
 """
+import weakref
+
 import torch
 import torch.nn as nn
 
@@ -288,11 +290,25 @@ class _SortedMoEFn(torch.autograd.Function):
         return (dx, dw, None, None, *grads)
 
 
+def _graph_release(layer):
+    """Hook for layer.balance_loss: once its gradient has come, the layer keeps the number."""
+    layer, loss = weakref.ref(layer), weakref.ref(layer.balance_loss)
+
+    def hook(_):
+        owner, done = layer(), loss()
+        if owner is not None and done is not None and owner.balance_loss is done:
+            owner.balance_loss = done.detach()
+
+    return hook
+
+
 class FusedMoEMLPSorted(nn.Module):
     """``balance_coef`` and ``z_coef`` (not in the reference; 0 leaves the layer as it was) ask
     for the routing's balance loss: each forward then leaves ``balance_loss`` = balance_coef *
     E sum_e f_e P_e + z_coef * mean(logsumexp^2) for the caller to add to its loss, and
-    ``expert_counts``, the tokens' slots per expert (int64 [E])."""
+    ``expert_counts``, the tokens' slots per expert (int64 [E]).  After its backward pass
+    ``balance_loss`` is the number alone: the layer keeps no graph alive (one that lives on from
+    an eager step would break the capture of a later step into a CUDA graph)."""
 
     def __init__(self, dim: int, hidden_dim: int, n_experts: int, k: int = 2,
                  router_version: str = "v2", balance_coef: float = 0.0, z_coef: float = 0.0):
@@ -374,6 +390,8 @@ class FusedMoEMLPSorted(nn.Module):
         if x_flat.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             raise TypeError(f"FusedMoEMLPSorted: unsupported dtype {x_flat.dtype}")
         x_flat = x_flat.contiguous()
+        if self.balance_coef > 0.0:
+            self.balance_loss = None  # the last graph goes before this one's nodes are made
         router_logits = self.router(x_flat)
         route_fn = fused_moe_route_v2 if self.router_version == "v2" else fused_moe_route
         topk_weights, topk_idx = route_fn(router_logits, self.k)
@@ -384,5 +402,7 @@ class FusedMoEMLPSorted(nn.Module):
                 logits, topk_idx, z_coef=self.z_coef / self.balance_coef,
                 loss_scale=self.balance_coef)
             self.balance_loss = loss * self.balance_coef
+            if self.balance_loss.requires_grad:
+                self.balance_loss.register_hook(_graph_release(self))
         out = _SortedMoEFn.apply(x_flat, topk_weights, topk_idx, self, *self._expert_params())
         return out.reshape(orig_shape)

@@ -183,3 +183,62 @@ def test_no_second_derivatives():
         (g,) = torch.autograd.grad(loss, x, create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             g.square().sum().backward()
+
+
+def captured_and_eager(step, params):
+    """Gradients of `step` run eagerly on the default stream, then captured and replayed."""
+    step()
+    eager = [p.grad.clone() for p in params]
+    for p in params:
+        p.grad = None
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for p in params:
+        p.grad.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    return eager, [p.grad for p in params], graph
+
+
+@pytest.mark.parametrize("backward", [True, False])
+def test_layer_keeps_no_graph(backward):
+    """After an eager step nothing of its graph lives on, so the next one can be captured."""
+    layer = FusedMoEMLPSorted(64, 64, 4, 2, balance_coef=0.01).cuda()
+    x = torch.randn(32, 64, device="cuda")
+    params = list(layer.parameters())
+
+    def step():
+        out = layer(x)
+        (out.square().mean() + layer.balance_loss).backward()
+
+    layer(x)
+    if backward:
+        step()
+        assert layer.balance_loss.grad_fn is None and not layer.balance_loss.requires_grad
+        assert float(layer.balance_loss) > 0.0
+        for p in params:
+            p.grad = None
+    eager, replayed, _ = captured_and_eager(step, params)
+    for a, b in zip(eager, replayed):
+        torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-8)
+
+
+def test_model_step_is_captured_after_an_eager_one():
+    model = make(fused_residual=True, n_experts=4)
+    x, y = (t.cuda() for t in batch())
+    params = list(model.parameters())
+
+    def step():
+        model(x, y).backward()
+
+    eager, replayed, graph = captured_and_eager(step, params)
+    for a, b in zip(eager, replayed):
+        torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-7)
+    assert float(model.balance_loss()) > 0.0
+    with torch.enable_grad():
+        model.logits(x)  # a forward alone, whose graph lives in the blocks
+    for p in params:
+        p.grad = None
+    captured_and_eager(step, params)
