@@ -75,6 +75,8 @@ class MLP(nn.Module):
 
 
 class Block(nn.Module):
+    fused_residual = False  # of a model that was pickled before it had the option
+
     def __init__(self, dim, n_heads, hidden_dim, fused: bool, fused_residual: bool = False,
                  n_experts: int = 0, k: int = 2, balance_coef: float = 0.0):
         super().__init__()
@@ -95,6 +97,8 @@ class Block(nn.Module):
 
 
 class MiniGPT(nn.Module):
+    fused_residual, n_experts = False, 0  # of a model that was pickled before it had the options
+
     def __init__(self, vocab_size=32000, dim=1024, n_layers=12, n_heads=16, hidden_dim=2752,
                  max_seq_len=1024, fused: bool = True, fused_residual: bool = False,
                  n_experts: int = 0, moe_k: int = 2, balance_coef: float = 0.01):

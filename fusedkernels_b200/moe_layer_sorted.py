@@ -310,6 +310,9 @@ class FusedMoEMLPSorted(nn.Module):
     ``balance_loss`` is the number alone: the layer keeps no graph alive (one that lives on from
     an eager step would break the capture of a later step into a CUDA graph)."""
 
+    # of a layer that was pickled before it had these
+    balance_coef, z_coef, balance_loss, expert_counts = 0.0, 0.0, None, None
+
     def __init__(self, dim: int, hidden_dim: int, n_experts: int, k: int = 2,
                  router_version: str = "v2", balance_coef: float = 0.0, z_coef: float = 0.0):
         super().__init__()
