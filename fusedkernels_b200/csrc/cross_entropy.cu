@@ -14,6 +14,7 @@
 // fixed-order reduction of the per-row losses (deterministic).  Rows that are not
 // 16-byte aligned use a scalar three-sweep kernel.
 #include "common.cuh"
+#include "exp.cuh"
 #include "ptx.cuh"
 
 #include <stdlib.h>
@@ -97,13 +98,6 @@ struct Online {
   float s;   // sum exp(x - m)
   float sx;  // sum x
 };
-
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T>
 __device__ __forceinline__ float exp_shift(float x, float m) {  // exp(x - m)

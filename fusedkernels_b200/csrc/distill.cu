@@ -718,6 +718,8 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
     const float hw = (row_state & kHard) ? a.hard_weight : 0.f;
     const float sw = (row_state & kSoft) ? 1.f - a.hard_weight : 0.f;
     const float ct = sw * a.temperature * a.loss_scale * inv_n, c1 = hw * a.loss_scale * inv_n;
+    // (2 ulp, as the exponentials they meet.  A full division and log2f keep more registers and
+    // spill: T = 2 842 against 816 us at 8192 x 128256 bf16, fp16 247 against 237 at 8192 x 32000.)
     const float kt = __fdividef(M != kOne ? ct : ct + c1, st.z);
     const float k1 = M != kOne ? __fdividef(c1, st.z1) : 0.f;
     const bool plain = row_state == kSkip || row_state == kBad;
