@@ -164,10 +164,11 @@ constexpr int fwd_groups(int tpr) { return tpr <= 32 ? 256 / tpr : 1; }
 // Forward, and with QUANT the 8-bit form (BLOCK: a scale per 128 columns, else per row).  TPR
 // threads take a row, thread t its chunks t, t + TPR, ...: every load of the row is in flight
 // before the first is used, the sum h stays in registers, and as the rows are independent the
-// SM hides one CTA's reduction under the others' loads.  Bound by HBM: 84 us forward, 76 us in 8
-// bits at 16384 x 4096 bf16 (6.4 and 6.2 TB/s).  As single elements 16 us at 5003 x 1111 bf16
-// with an fp32 residual (4.2 TB/s; the element loops below 29, whole-line tiles through shared
-// memory 32: too few rows in flight).
+// SM hides one CTA's reduction under the others' loads.  Bound by HBM: 84 us forward at
+// 16384 x 4096 bf16 (6.4 TB/s); in 8 bits 79 us per 128 columns and 82 per row (5.9 and 5.7 TB/s:
+// the quotients take the kernel to 85% of the issue slots).  As single elements 16 us at
+// 5003 x 1111 bf16 with an fp32 residual (4.2 TB/s; the element loops below 29, whole-line tiles
+// through shared memory 32: too few rows in flight), in 8 bits 27 (one byte a store).
 template <typename T, typename R, int VN, int TPR, int CPT, bool QUANT, bool BLOCK>
 __global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR) add_rmsnorm_rows(
     const T* __restrict__ x, int64_t xs, const R* __restrict__ r, int64_t rs,
@@ -340,7 +341,7 @@ bool rows_of_chunks(const FwdArgs& a) {
 
 // Runs the chunk kernel where the rows allow it (at most 2048 chunks); -1 where they do not.
 // 256 threads of 2 chunks beat 128 of 4 at 16384 x 4096 bf16 (forward 83.9 against 85.3 us, 8
-// bits 75.1 against 77.3); where 128 threads of 3 suffice, they hold more rows at a time.
+// bits, before their quotients were corrected, 75.1 against 77.3); where 128 threads of 3 suffice, they hold more rows at a time.
 template <typename T, typename R, bool QUANT, bool BLOCK>
 int rows_chunked(const FwdArgs& a, cudaStream_t st) {
   if (!rows_of_chunks<T, R>(a)) return -1;
@@ -405,7 +406,7 @@ __device__ __forceinline__ void bwd_store(const Chunk<T, VN>& dy, const Chunk<R,
   if (sizeof(T) != sizeof(R)) orr.store(dr);
 }
 
-// Rows of at most 128 chunks: TPR lanes of a warp take a row (no CTA barrier per row), and the
+// Rows of at most 64 chunks: TPR lanes of a warp take a row (no CTA barrier per row), and the
 // next row is loaded while this one is worked on.
 template <typename T, typename R, int TPR, int CPT>
 __global__ void __launch_bounds__(256) add_rmsnorm_bwd_lanes(BwdArgs a) {
@@ -497,8 +498,10 @@ __global__ void __launch_bounds__(256) add_rmsnorm_bwd_lanes(BwdArgs a) {
 // Longer rows: the CTA takes a row.  Rows of dy, h and dh arrive in a ring of shared-memory
 // stages by cp.async.bulk; a stage is refilled as soon as all threads have its chunks in
 // registers, which the reduction's barrier tells.  Bound by HBM: 86 us at 16384 x 4096 bf16 (6.3
-// TB/s), 4 us more for dw.  Stages: 3 where they take 72 KB (three CTAs an SM), else 2, or 1.
-constexpr int kBwdMaxStages = 4;
+// TB/s), 4 us more for dw.  Stages: 3 where they take 72 KB (three CTAs an SM), else 2, or 1.  At
+// 4096 x 16384 bf16 96 us for 83 of bytes, 48 bytes spilled; with an fp32 stream a stage is 160 KB, so
+// one CTA an SM holds one stage, and 176 bytes are spilled: 212 us for 166.
+constexpr int kBwdMaxStages = 3;
 template <typename T, typename R, int THREADS, int CPT>
 __global__ void __launch_bounds__(THREADS) add_rmsnorm_bwd_ring(BwdArgs a, int stages) {
   constexpr int VN = 16 / (int)sizeof(T);
@@ -671,7 +674,8 @@ int bwd_chunked(const BwdArgs& a, int* grid, cudaStream_t st) {
 // ------------------------------------------------------------------ backward, columns ---
 // Rows of any width, stride and alignment: thread t of the CTA has the columns t, t + THREADS,
 // ... as single elements, the next row's on their way while this one is worked on.  22 us at
-// 5003 x 1111 bf16 with an fp32 residual (element loops 54, tiles through shared memory 40).
+// 5003 x 1111 bf16 with an fp32 residual (element loops 54, tiles through shared memory 40).  Above
+// 4096 columns 208 to 268 bytes are spilled: 90 us at 4096 x 8191 bf16 for 42 of bytes.
 template <typename T, typename R, int THREADS, int CPT>
 __global__ void __launch_bounds__(THREADS) add_rmsnorm_bwd_columns(BwdArgs a) {
   __shared__ float red[2][32];
@@ -763,7 +767,9 @@ int bwd_columns(const BwdArgs& a, int* grid, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ any shape -----------
-// One CTA per row, element loops.  h is re-read by the thread that wrote it.
+// One CTA per row, element loops.  h is re-read by the thread that wrote it.  At 1677 x 40000 bf16
+// forward 277 us, backward 651 and 47 for dw, for 83 of bytes each; in 8 bits 392 per row and 906 per
+// 128 columns for 73.
 template <typename T, typename R>
 __global__ void __launch_bounds__(256) add_rmsnorm_fwd_generic(
     const T* __restrict__ x, int64_t xs, const R* __restrict__ r, int64_t rs,

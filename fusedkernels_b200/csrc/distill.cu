@@ -312,7 +312,8 @@ __device__ __forceinline__ void finish_loss(const RowArgs& a, double mine) {
 // ------------------------------------------------------------------ rows, any layout ----
 constexpr int kGenericThreads = 256;
 
-// One CTA per row, element loops (any stride, alignment and length).
+// One CTA per row, element loops (any stride, alignment and length).  Three passes over the row: 3.1
+// ms at 2048 x 262144 bf16 for 0.33 of bytes, 0.97 ms at 1024 x 151936 fp32 for 0.19.
 template <typename T>
 __global__ void __launch_bounds__(kGenericThreads) distill_rows_generic(
     const T* logits, int64_t lstride, T* grad, int64_t gstride, RowArgs a) {
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(kGenericThreads) distill_rows_generic(
 // exchange (m, z) by st.async into each other's shared memory.  16-bit packets stay in
 // registers and the gradient's exponentials are formed anew: keeping the first ones in 32 bits
 // takes twice the registers, half as many rows are then in flight, and their latency shows
-// (810 against 717 us at 8192 x 128256 bf16).  32-bit packets give their registers to their
+// (810 against 717 us at 8192 x 128256 bf16, before x - max was formed; 725 since).  32-bit packets give their registers to their
 // exponentials, which the gradient only scales.
 //
 // Elements before the first and after the last 16-byte boundary of a row (any odd width or
@@ -445,8 +446,10 @@ union PairPacket {
 
 // What a row needs: softmax at one temperature, or at two (the soft part's, T, and 1).  Where T
 // is a ratio of small numbers P / Q, one exponential b = exp(d / P) gives both: b^Q = exp(d / T)
-// and b^P = exp(d).  kSquare is T = 2, kPowers T = 3, 4 and 3 / 2 (at 4096 x 128256 bf16: one
-// temperature 362 us, T = 2 386, two exponentials per logit 722).
+// and b^P = exp(d), with Q and P times b's relative error (2 to 3 ulp).  kSquare is T = 2,
+// kPowers T = 3, 4 and 3 / 2.  At 8192 x 128256 bf16 (651 us of bytes): one temperature 725 us, T = 2
+// 749, kPowers 950, two exponentials per logit (T = 2.5) 1451: the ex2 unit alone takes 900 for them, and
+// 280 bytes are spilled.  At 2048 x 50257 fp32 (128 us of bytes): T = 2 149, T = 3 228, T = 2.5 285.
 enum Mode { kOne, kTwo, kSquare, kPowers };
 
 // (maximum, sum exp((x - max) / T), sum exp(x - max)) of a set of logits.
@@ -907,7 +910,8 @@ int launch_rows(const T* lp, int64_t ls, T* gp, int64_t gs, int log_c, int stage
   cfg.gridDim = dim3((unsigned)((clusters < 1 ? 1 : clusters) * cluster));
   // The kernel may start, and load its first rows, while the teacher kernel ends.  Not so a
   // grid of clusters that fills the GPU: placed among the teacher's last CTAs it finds no room
-  // for all its clusters at once, and the rest runs as a second wave (1186 against 717 us).
+  // for all its clusters at once, and the rest runs as a second wave (1186 against 717 us at
+  // 8192 x 128256 bf16).
   if (cluster == 1 || 2 * clusters <= most) {
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -922,8 +926,9 @@ template <typename T, Mode M>
 int rows_mode(const T* lp, int64_t ls, T* gp, int64_t gs, const RowArgs& a, cudaStream_t st) {
   // Cluster: as many CTAs as a row needs for slices of at most 32 KB (64 KB where 8 do not
   // suffice), more (down to 8 KB) while the rows are too few for the SMs.  128 threads of 16
-  // packets and 4 such CTAs per SM measured best at 8192 x 128256 bf16: 717 us, against 809 with
-  // 256 threads and half the CTAs per row, 942 with 256 threads of 8 packets.
+  // packets and 4 such CTAs per SM measured best at 8192 x 128256 bf16: 717 us (725 since x - max
+  // is formed), against 809 with 256 threads and half the CTAs per row, 942 with 256 threads of 8
+  // packets.
   const int64_t packets = (int64_t)a.n_cols * sizeof(T) / 16 + 1;
   int lc = 0;
   while (lc < 3 && packets > (int64_t)2048 << lc) ++lc;
@@ -970,7 +975,9 @@ int teacher_t(const int64_t* idx, const void* top, int k, const int64_t* targets
   int log_table = 5;
   while ((1 << log_table) < 2 * k) ++log_table;
   // Many short rows: 8 lanes a row, so that the reductions of 4 rows are one instruction.  Few
-  // or long ones: a warp a row.
+  // or long ones: a warp a row.  8 lanes against a warp, us: 8192 rows of 16 5.7 / 7.9, 8192 of 64
+  // 11.3 / 10.4, 32768 of 64 24.9 / 33.5; 2048 of 16 5.3 / 5.0, 2048 of 64 10.0 / 6.1, 8192 of 100
+  // 15.4 / 15.2; at the edge itself, 4096 of 64, 10.5 / 7.4.
   const bool narrow = n_rows >= 4096 && k <= 64;
   const int rows = kTeacherWarps * (narrow ? 4 : 1);
   const int smem = rows * row_ints(k, log_table) * 4;

@@ -82,8 +82,9 @@ def fused_distillation_loss(logits: torch.Tensor, teacher_idx: torch.Tensor,
     where no gradient is wanted the logits are left as they are.
     loss_scale: the factor that the backward pass will be started with (a GradScaler's scale).
     It is folded into the gradient in 32 bits, before the rounding to the logits' dtype; any
-    other factor gives the right gradient too, at one more pass over it.  The returned loss is
-    not scaled.  The gradient is handed over once: a second backward pass through the same
+    other factor gives the right gradient too, at one more pass over it and within what the
+    logits' dtype held before (in fp16 what has overflowed or vanished stays so).  The returned
+    loss is not scaled.  The gradient is handed over once: a second backward pass through the same
     graph raises.
 
     A teacher id or target >= V (or a negative target that is not ignore_index) makes the loss

@@ -59,15 +59,16 @@ def fused_moe_balance_loss(router_logits: torch.Tensor, topk_idx: torch.Tensor,
     fp32 loss (see the module's docstring) and int64 counts [E].
 
     router_logits: [N, E] fp32, fp16 or bf16, E <= 256.  topk_idx: [N, k] expert indices as
-    the routers return them; a negative one is an unused slot, one >= E makes the loss and its
-    gradient NaN.  token_mask: [N] bool; tokens that are False (padding) count nowhere and get
-    a zero gradient.  With no counted token the loss is 0.  A token whose logits are all -inf
-    has no probabilities: it adds 0 to both sums.
+    the routers return them; a negative one is an unused slot, one >= E in a counted token makes
+    the loss and the whole gradient NaN.  token_mask: [N] bool; tokens that are False (padding)
+    count nowhere and get a zero gradient.  With no counted token the loss is 0.  A token whose
+    logits are all -inf has no probabilities: it adds 0 to both sums.
 
     loss_scale: the factor that the backward pass will be started with (a GradScaler's scale,
     or the weight the loss is added with).  It is folded into the gradient in 32 bits, before
     the rounding to the logits' dtype; any other factor gives the right gradient too, at one
-    more pass over it.  The returned loss is not scaled.  The gradient is handed over once: a
+    more pass over it and within what the logits' dtype held before (in fp16 what has overflowed
+    or vanished stays so).  The returned loss is not scaled.  The gradient is handed over once: a
     second backward pass through the same graph raises."""
     assert router_logits.is_cuda and router_logits.ndim == 2
     n_rows, n_experts = router_logits.shape
