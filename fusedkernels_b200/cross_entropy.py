@@ -67,7 +67,10 @@ def fused_cross_entropy(logits: torch.Tensor, targets: torch.Tensor,
                         ignore_index: int = -100, label_smoothing: float = 0.0,
                         inplace_grad: bool = False) -> torch.Tensor:
     """Drop-in fused replacement for F.cross_entropy(logits, targets).
-    logits: [N, V], targets: [N] long. Returns scalar mean loss."""
+    logits: [N, V], targets: [N] long. Returns scalar mean loss.
+    16-bit logits: the running maximum is folded into the exponents, which puts an error of about
+    |max| * 2^-24 into a row's loss and makes it NaN beside logits masked with bf16's lowest value:
+    mask with -inf."""
     return _FusedCrossEntropy.apply(logits, targets, ignore_index, label_smoothing, inplace_grad)
 
 

@@ -50,11 +50,11 @@ __device__ __forceinline__ float block_max(float v, float* red) {
 }
 
 // The 8-bit form divides twice: scale = m / 448 for a group's largest magnitude m, and y / scale.
-// Products with a reciprocal are off by up to 3 steps, and beside an e4m3 tie that moves a value to
-// the other neighbour, a step of up to 1/8 of it.  The residual r = q b - a of such a quotient q
-// of a / b is an FMA without error (or next to none), and puts it right (Markstein 1990): q - r / b is off
-// by 2^-20 steps before its one rounding, and keeps the sign of a zero.  (A call at 16384 x 4096
-// bf16, per 128: 79 us with the bare products, 80 so, 97 with divisions.)
+// Products with a reciprocal are off by up to 3 steps, and beside an e4m3 tie that moves a value
+// to the other neighbour, a step of up to 1/8 of it.  The residual r = q b - a of such a quotient
+// q of a / b is an FMA without error (or next to none), and puts it right (Markstein 1990):
+// q - r / b is off by 2^-20 steps before its one rounding, and keeps the sign of a zero.  (A call at
+// 16384 x 4096 bf16, per 128: 79 us with the bare products, 80 so, 97 with divisions.)
 __device__ __forceinline__ float divide(float a, float b, float inv_b) {
   const float q = a * inv_b;
   return fmaf(-fmaf(q, b, -a), inv_b, q);
@@ -66,7 +66,8 @@ __device__ __forceinline__ float scale_of(float m) {
 }
 
 // y / scale for the values of a group: of both times a power of two, exactly, where scale is so
-// small that residuals would leave the normal range.  (Beside an infinite value q is 0, as by a division.)
+// small that residuals would leave the normal range.  (Beside an infinite value q is 0, as by a
+// division.)
 struct Quotient {
   float by, b, inv;
   __device__ __forceinline__ explicit Quotient(float scale)
@@ -339,9 +340,10 @@ bool rows_of_chunks(const FwdArgs& a) {
          a.rows < ((int64_t)1 << 31);
 }
 
-// Runs the chunk kernel where the rows allow it (at most 2048 chunks); -1 where they do not.
-// 256 threads of 2 chunks beat 128 of 4 at 16384 x 4096 bf16 (forward 83.9 against 85.3 us, 8
-// bits, before their quotients were corrected, 75.1 against 77.3); where 128 threads of 3 suffice, they hold more rows at a time.
+// Runs the chunk kernel where the rows allow it (at most 2048 chunks); -1 where they do not.  256
+// threads of 2 chunks beat 128 of 4 at 16384 x 4096 bf16 (forward 83.9 against 85.3 us, 8 bits,
+// before their quotients were corrected, 75.1 against 77.3); where 128 threads of 3 suffice, they
+// hold more rows at a time.
 template <typename T, typename R, bool QUANT, bool BLOCK>
 int rows_chunked(const FwdArgs& a, cudaStream_t st) {
   if (!rows_of_chunks<T, R>(a)) return -1;
@@ -495,12 +497,12 @@ __global__ void __launch_bounds__(256) add_rmsnorm_bwd_lanes(BwdArgs a) {
     a.part[(int64_t)blockIdx.x * a.cols + c] = sum[c];
 }
 
-// Longer rows: the CTA takes a row.  Rows of dy, h and dh arrive in a ring of shared-memory
-// stages by cp.async.bulk; a stage is refilled as soon as all threads have its chunks in
-// registers, which the reduction's barrier tells.  Bound by HBM: 86 us at 16384 x 4096 bf16 (6.3
-// TB/s), 4 us more for dw.  Stages: 3 where they take 72 KB (three CTAs an SM), else 2, or 1.  At
-// 4096 x 16384 bf16 96 us for 83 of bytes, 48 bytes spilled; with an fp32 stream a stage is 160 KB, so
-// one CTA an SM holds one stage, and 176 bytes are spilled: 212 us for 166.
+// Longer rows: the CTA takes a row.  Rows of dy, h and dh arrive in a ring of shared-memory stages
+// by cp.async.bulk; a stage is refilled as soon as all threads have its chunks in registers, which
+// the reduction's barrier tells.  Bound by HBM: 86 us at 16384 x 4096 bf16 (6.3 TB/s), 4 us more
+// for dw.  Stages: 3 where they take 72 KB (three CTAs an SM), else 2, or 1.  At 4096 x 16384 bf16
+// 96 us for 83 of bytes, 48 bytes spilled; with an fp32 stream a stage is 160 KB, so one CTA an SM
+// holds one stage, and 176 bytes are spilled: 212 us for 166.
 constexpr int kBwdMaxStages = 3;
 template <typename T, typename R, int THREADS, int CPT>
 __global__ void __launch_bounds__(THREADS) add_rmsnorm_bwd_ring(BwdArgs a, int stages) {
@@ -768,8 +770,8 @@ int bwd_columns(const BwdArgs& a, int* grid, cudaStream_t st) {
 
 // ------------------------------------------------------------------ any shape -----------
 // One CTA per row, element loops.  h is re-read by the thread that wrote it.  At 1677 x 40000 bf16
-// forward 277 us, backward 651 and 47 for dw, for 83 of bytes each; in 8 bits 392 per row and 906 per
-// 128 columns for 73.
+// forward 277 us, backward 651 and 47 for dw, for 83 of bytes each; in 8 bits 392 per row and 906
+// per 128 columns for 73.
 template <typename T, typename R>
 __global__ void __launch_bounds__(256) add_rmsnorm_fwd_generic(
     const T* __restrict__ x, int64_t xs, const R* __restrict__ r, int64_t rs,

@@ -271,10 +271,10 @@ struct Args {
 };
 
 // Rows are read ahead: the next ones are on their way while these are worked on, and the first
-// ones while the counting kernel ends.  At 131072 x 128 fp32 25 us by itself, 32 from its
-// start under the count (its floor is 21: the copy rate); 62% of the issue slots, 26 instructions a
-// logit and warp, so it is bound by both.  Count and rows together there: 37 us with three CTAs an SM
-// (24 bytes spilled), 37 with two (none), 43 with four.
+// ones while the counting kernel ends.  At 131072 x 128 fp32 25 us by itself, 32 from its start
+// under the count (its floor is 21: the copy rate); 62% of the issue slots, 26 instructions a
+// logit and warp, so it is bound by both.  Count and rows together there: 37 us with three CTAs an
+// SM (24 bytes spilled), 37 with two (none), 43 with four.
 template <typename T, Layout LAYOUT, int L, int PP>
 constexpr int ctas_per_sm() {  // by the registers that a lane's logits take
   const int values = LAYOUT == kPacked ? PP * 16 / (int)sizeof(T) : LAYOUT == kTiled ? 4 * PP : PP;

@@ -312,8 +312,8 @@ __device__ __forceinline__ void finish_loss(const RowArgs& a, double mine) {
 // ------------------------------------------------------------------ rows, any layout ----
 constexpr int kGenericThreads = 256;
 
-// One CTA per row, element loops (any stride, alignment and length).  Three passes over the row: 3.1
-// ms at 2048 x 262144 bf16 for 0.33 of bytes, 0.97 ms at 1024 x 151936 fp32 for 0.19.
+// One CTA per row, element loops (any stride, alignment and length).  Three passes over the row:
+// 3.1 ms at 2048 x 262144 bf16 for 0.33 of bytes, 0.97 ms at 1024 x 151936 fp32 for 0.19.
 template <typename T>
 __global__ void __launch_bounds__(kGenericThreads) distill_rows_generic(
     const T* logits, int64_t lstride, T* grad, int64_t gstride, RowArgs a) {
@@ -395,8 +395,8 @@ __global__ void __launch_bounds__(kGenericThreads) distill_rows_generic(
 // exchange (m, z) by st.async into each other's shared memory.  16-bit packets stay in
 // registers and the gradient's exponentials are formed anew: keeping the first ones in 32 bits
 // takes twice the registers, half as many rows are then in flight, and their latency shows
-// (810 against 717 us at 8192 x 128256 bf16, before x - max was formed; 725 since).  32-bit packets give their registers to their
-// exponentials, which the gradient only scales.
+// (810 against 717 us at 8192 x 128256 bf16, before x - max was formed; 725 since).  32-bit packets
+// give their registers to their exponentials, which the gradient only scales.
 //
 // Elements before the first and after the last 16-byte boundary of a row (any odd width or
 // offset) are taken singly by the first CTA.  Logits and gradient have to have the same
@@ -444,12 +444,13 @@ union PairPacket {
   __device__ __forceinline__ PairPacket() {}
 };
 
-// What a row needs: softmax at one temperature, or at two (the soft part's, T, and 1).  Where T
-// is a ratio of small numbers P / Q, one exponential b = exp(d / P) gives both: b^Q = exp(d / T)
-// and b^P = exp(d), with Q and P times b's relative error (2 to 3 ulp).  kSquare is T = 2,
-// kPowers T = 3, 4 and 3 / 2.  At 8192 x 128256 bf16 (651 us of bytes): one temperature 725 us, T = 2
-// 749, kPowers 950, two exponentials per logit (T = 2.5) 1451: the ex2 unit alone takes 900 for them, and
-// 280 bytes are spilled.  At 2048 x 50257 fp32 (128 us of bytes): T = 2 149, T = 3 228, T = 2.5 285.
+// What a row needs: softmax at one temperature, or at two (the soft part's, T, and 1).  Where T is
+// a ratio of small numbers P / Q, one exponential b = exp(d / P) gives both: b^Q = exp(d / T) and
+// b^P = exp(d), with Q and P times b's relative error (2 to 3 ulp).  kSquare is T = 2, kPowers T =
+// 3, 4 and 3 / 2.  At 8192 x 128256 bf16 (651 us of bytes): one temperature 725 us, T = 2 749,
+// kPowers 950, two exponentials per logit (T = 2.5) 1451: the ex2 unit alone takes 900 for them,
+// and 280 bytes are spilled.  At 2048 x 50257 fp32 (128 us of bytes): T = 2 149, T = 3 228, T =
+// 2.5 285.
 enum Mode { kOne, kTwo, kSquare, kPowers };
 
 // (maximum, sum exp((x - max) / T), sum exp(x - max)) of a set of logits.
@@ -635,8 +636,9 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) distill_rows(
       my_m = fmaxf(fmaxf(f.x, f.y), xs);
     }
     const float base = my_m == -INFINITY ? 0.f : my_m;
-    // The maximum goes off first: folded into the exponent as the constant -max log2(e) / T it would
-    // leave that product's rounding in every term, and overflow at a mask of the type's lowest value.
+    // The maximum goes off first: folded into the exponent as the constant -max log2(e) / T it
+    // would leave that product's rounding in every term, and overflow at a mask of the type's
+    // lowest value.
     auto exp_one = [&](float x, float& f, float& f1) {
       const float d = x - base;
       if constexpr (sizeof(T) == 2) {

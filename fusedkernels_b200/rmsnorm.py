@@ -159,8 +159,9 @@ def fused_add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None,
     ``block=None`` gives one fp32 scale per row (scales [..., 1]), ``block=128`` one per 128
     columns (scales [..., ceil(cols / 128)]): max|y| / 448 over the group, at least 2^-126.  The
     32-bit ``y`` is quantised, so it is rounded once; quotients that are ties of e4m3 in exact
-    arithmetic (those of 16-bit values often are) go by the last bit of that ``y``.  It is a forward for inference and for the
-    8-bit side of a product: it has no gradient, and asserts that none is asked for."""
+    arithmetic (those of 16-bit values often are) go by the last bit of that ``y``.  It is a
+    forward for inference and for the 8-bit side of a product: it has no gradient, and asserts
+    that none is asked for."""
     _check_add_norm(x, residual, weight)
     assert block in (None, 128), "block is None (a scale per row) or 128"
     assert not _lib.wants_derivative(x, weight, *(() if residual is None else (residual,))), \
